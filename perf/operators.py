@@ -1,0 +1,223 @@
+"""The 8-bit activation path's operators, as cases that can be timed and compared.
+
+Three operators that a layer of the trunk runs one after the other when its activations are held in int8 with one float32 scale a token:
+
+* `rms_norm_s8`: the residual's addition and the zero-centred RMS norm, leaving int8 rows and their scales;
+* `quantize_tokens_s8`: the same last step for activations that no norm makes (a mixer's output, the SwiGLU's);
+* `gemm_s8`: the product of int8 activations and int8 weights, one scale a token and one a weight row, with the projections' epilogues.
+
+The rows of a call are one token that continues a request, a short line, an alert of 900 tokens, up to a full call of 4096.
+"""
+from __future__ import annotations
+
+import torch
+
+own = False  # set from outside: False, the operators in elementary torch operations; True, the framework's calls
+
+CALL_ROWS = 4096
+EPS = 1e-6
+
+HIDDEN = [1024, 2048, 2560, 4096]               # hidden sizes of the served models and the 36-layer stack
+INNER = [2048, 3584, 4096, 6144, 9728, 12288]   # mixer outputs and SwiGLU widths
+# (N, K, epilogue) of the projections of the same models, and a small odd pair
+PROJECTIONS = [
+    (19456, 2560, "swiglu"), (9728, 2560, "store"), (2560, 9728, "add"), (6144, 2560, "store"), (1024, 2560, "store"), (2560, 4096, "add"),
+    (8192, 2560, "store"), (2560, 2048, "add"), (7168, 1024, "swiglu"), (1024, 3584, "add"), (24576, 4096, "swiglu"), (4096, 12288, "add"),
+    (1000, 1360, "store"),
+]
+
+
+def listed():
+    return [
+        # one more token of a request, the smallest model: a launch's latency is all there is
+        {"name": "norm, one token", "kind": "norm", "t": 1, "c": 1024, "delta": "none", "smooth": False},
+        # an alert through the 36-layer stack, the mixer's output (binary16) still to be added to the stream
+        {"name": "norm, alert", "kind": "norm", "t": 900, "c": 2560, "delta": "half", "smooth": False},
+        # a full call of the largest model, columns smoothed, the addition done by the projection before
+        {"name": "norm, full call", "kind": "norm", "t": 4096, "c": 4096, "delta": "none", "smooth": True},
+        # a short line's SwiGLU output
+        {"name": "quantise, short line", "kind": "quantise", "t": 29, "c": 3584, "half": True, "smooth": False, "band": 0},
+        # an alert's mixer output, a band of a wider buffer
+        {"name": "quantise, alert's band", "kind": "quantise", "t": 901, "c": 4096, "half": True, "smooth": False, "band": 4096},
+        # the widest SwiGLU output of a full call, float32
+        {"name": "quantise, full call", "kind": "quantise", "t": 4096, "c": 12288, "half": False, "smooth": True, "band": 0},
+        # the fused q, k, v projection of one token: reading the weights once
+        {"name": "qkv, one token", "kind": "gemm", "t": 1, "n": 6144, "k": 2560, "epilogue": "store", "half": True},
+        # the down projection of a short line, added to the stream
+        {"name": "down, short line", "kind": "gemm", "t": 29, "n": 2560, "k": 9728, "epilogue": "add", "half": False},
+        # the down projection of an alert
+        {"name": "down, alert", "kind": "gemm", "t": 900, "n": 2560, "k": 9728, "epilogue": "add", "half": False},
+        # an odd number of rows into the fused q, k, v projection
+        {"name": "qkv, odd rows", "kind": "gemm", "t": 1337, "n": 6144, "k": 2560, "epilogue": "store", "half": True},
+        # the alert's gate and up, SwiGLU fused
+        {"name": "gate and up, alert", "kind": "gemm", "t": 900, "n": 19456, "k": 2560, "epilogue": "swiglu", "half": True},
+        # the widest product of a full call of the largest model
+        {"name": "gate and up, full call", "kind": "gemm", "t": 4096, "n": 24576, "k": 4096, "epilogue": "swiglu", "half": True},
+    ]
+
+
+def _spread(rng, low, high):
+    """A whole number between low and high, even over the logarithm."""
+    return max(low, min(high, int(round(low * (high / low) ** rng.random()))))
+
+
+def draw(rng):
+    kind = rng.choice(["norm", "quantise", "gemm", "gemm"])
+    t = _spread(rng, 1, CALL_ROWS)
+    if kind == "norm":
+        return {"kind": kind, "t": t, "c": rng.choice(HIDDEN), "delta": rng.choice(["none", "half", "float"]), "smooth": rng.random() < 0.3}
+    if kind == "quantise":
+        return {"kind": kind, "t": t, "c": rng.choice(INNER), "half": rng.random() < 0.7, "smooth": rng.random() < 0.3, "band": rng.choice([0, 0, 64, 2048])}
+    n, k, epilogue = rng.choice(PROJECTIONS)
+    return {"kind": kind, "t": t, "n": n, "k": k, "epilogue": epilogue, "half": epilogue != "add" and rng.random() < 0.7}
+
+
+def _normal(gen, *shape, std=1.0):
+    return torch.randn(shape, generator=gen, device="cuda") * std
+
+
+def _activations(gen, t, c):
+    """Rows as a residual stream has them: a scale of its own for each row, and a few columns that stand far out."""
+    v = _normal(gen, t, c) * (0.25 + 4.0 * torch.rand((t, 1), generator=gen, device="cuda"))
+    v[:, :: max(1, c // 8)] *= 12.0
+    return v
+
+
+def _to_bytes(v):
+    top = v.abs().amax(1, keepdim=True)
+    return torch.round(v * (127.0 / top)).clamp(-127, 127).to(torch.int8), (top / 127.0).reshape(-1)
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    t = case["t"]
+    state = dict(case)
+    if case["kind"] == "gemm":
+        n, k = case["n"], case["k"]
+        state["xq"], state["sx"] = _to_bytes(_activations(gen, t, k))
+        state["wq"], state["sw"] = _to_bytes(_normal(gen, n, k, std=0.02))  # placed once: the layout of the int8 weights with a scale a row
+        columns = n // 2 if case["epilogue"] == "swiglu" else n
+        kind = torch.float16 if case["half"] else torch.float32
+        state["y"] = _normal(gen, t, columns).to(kind) if case["epilogue"] == "add" else torch.empty((t, columns), dtype=kind, device="cuda")
+    else:
+        c = case["c"]
+        state["smooth"] = torch.exp(_normal(gen, c, std=0.3)) if case["smooth"] else None
+        if case["kind"] == "norm":
+            state["x"] = _activations(gen, t, c)
+            state["w"] = _normal(gen, c, std=0.2)
+            # the sum added by every pass is small beside the stream
+            state["delta"] = None if case["delta"] == "none" else _normal(gen, t, c, std=0.3).to(torch.float16 if case["delta"] == "half" else torch.float32)
+        else:
+            kind = torch.float16 if case["half"] else torch.float32
+            state["x"] = _activations(gen, t, c + case["band"]).to(kind)[:, :c]
+        state["q"] = torch.empty((t, c), dtype=torch.int8, device="cuda")
+        state["scales"] = torch.empty((t,), device="cuda")
+        state["by_row"] = state["scales"].view(t, 1)
+        state["values"] = torch.empty((t, c), dtype=torch.float16, device="cuda")
+    return state
+
+
+_ctx = None
+
+
+def _context():
+    """The library and a program's context on it, opened once and kept. (The plain forms never come here: they run on trees that lack the operators.)"""
+    global _ctx
+    import sepal_runner_b200 as sb
+
+    if _ctx is None:
+        _ctx = sb.Context(0)
+        _ctx.set_static_weights(True)  # the weights are placed once, before the first call
+    return sb, _ctx
+
+
+def run(state):
+    if state["kind"] == "gemm":
+        return _run_gemm(state)
+    if own:
+        _, ctx = _context()
+        if state["kind"] == "norm":
+            ctx.rms_norm_s8(state["x"], state["w"], state["q"], state["scales"], delta=state["delta"], col_scale=state["smooth"], eps=EPS)
+        else:
+            ctx.quantize_tokens_s8(state["x"], state["q"], state["scales"], col_scale=state["smooth"])
+        # the values that the bytes stand for
+        out = {"values": torch.mul(state["q"], state["by_row"], out=state["values"]), "scales": state["scales"]}
+    else:
+        x = state["x"]
+        if state["kind"] == "norm":
+            if state["delta"] is not None:
+                x.add_(state["delta"].float())
+            v = x * torch.rsqrt((x * x).mean(1, keepdim=True) + EPS) * (1.0 + state["w"])
+        else:
+            v = x.float()
+        if state["smooth"] is not None:
+            v = v * state["smooth"]
+        top = v.abs().amax(1, keepdim=True)
+        scales = top / 127.0
+        q = torch.round(v * torch.where(top > 0, 127.0 / top, 0.0)).clamp(-127.0, 127.0)
+        out = {"values": (q * scales).to(torch.float16), "scales": scales.reshape(-1)}
+    if state["kind"] == "norm" and state["delta"] is not None:
+        out["x"] = state["x"]
+    return out
+
+
+def _run_gemm(state):
+    y = state["y"]
+    if own:
+        sb, ctx = _context()
+        epilogue = {"store": sb.STORE, "add": sb.ADD, "swiglu": sb.SWIGLU}[state["epilogue"]]
+        return ctx.gemm_s8(state["xq"], state["sx"], state["wq"], state["sw"], y, epilogue=epilogue)
+    sums = (state["xq"].float() @ state["wq"].float().T) * state["sx"][:, None] * state["sw"]
+    if state["epilogue"] == "add":
+        return y.copy_(y.float() + sums)
+    if state["epilogue"] == "swiglu":
+        blocks = sums.view(sums.shape[0], -1, 2, 64)  # weight rows: 64 of gate, 64 of up, in turn
+        gate, up = blocks[:, :, 0], blocks[:, :, 1]
+        sums = (gate / (1.0 + torch.exp(-gate)) * up).reshape(sums.shape[0], -1)
+    return sums.to(y.dtype)
+
+
+def work(case):
+    t = case["t"]
+    if case["kind"] == "gemm":
+        n, k = case["n"], case["k"]
+        columns = n // 2 if case["epilogue"] == "swiglu" else n
+        size = 2 if case["half"] else 4
+        passes = 2 if case["epilogue"] == "add" else 1
+        return {"bytes": t * k + n * k + 4 * (t + n) + passes * size * t * columns, "flops": 2 * t * n * k}
+    c = case["c"]
+    # each value returned is a byte (and the row's scale) in the operator's own output
+    row = {"norm": 4, "quantise": 2 if case.get("half") else 4}[case["kind"]] + 1
+    if case["kind"] == "norm":
+        row += {"none": 0, "half": 2 + 4, "float": 4 + 4}[case["delta"]]
+    columns = 4 * c * ((case["kind"] == "norm") + bool(case["smooth"]))
+    return {"bytes": t * c * row + 4 * t + columns, "flops": t * c * (8 if case["kind"] == "norm" else 3)}
+
+
+def exact(case, seed):
+    """From the definitions, in 64 bits."""
+    s = prepare(case, seed)
+    if case["kind"] == "gemm":
+        acc = torch.einsum("tk,nk->tn", s["xq"].double(), s["wq"].double())
+        acc = torch.einsum("tn,t,n->tn", acc, s["sx"].double(), s["sw"].double())
+        if case["epilogue"] == "add":
+            return s["y"].double() + acc
+        if case["epilogue"] == "swiglu":
+            rows = torch.arange(case["n"], device="cuda")
+            gate, up = acc[:, rows % 128 < 64], acc[:, rows % 128 >= 64]
+            return torch.sigmoid(gate) * gate * up
+        return acc
+    v = s["x"].double()
+    out = {}
+    if case["kind"] == "norm":
+        if s["delta"] is not None:
+            # the stream is held in float32: what is normalised is the sum that was stored
+            v = (v + s["delta"].double()).float().double()
+            out["x"] = v
+        v = v / (v.square().sum(1, keepdim=True) / case["c"] + EPS).sqrt() * (s["w"].double() + 1.0)
+    if s["smooth"] is not None:
+        v = v * s["smooth"].double()
+    step = v.abs().max(dim=1, keepdim=True).values / 127.0
+    whole = torch.where(step > 0, v / step, 0.0).round().clamp(-127, 127)
+    out["values"], out["scales"] = whole * step, step[:, 0]
+    return out
