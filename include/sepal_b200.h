@@ -174,6 +174,43 @@ SEPAL_B200_API int32_t sepal_b200_gemm_w8r(sepal_b200_ctx* ctx, const void* x, u
 SEPAL_B200_API int32_t sepal_b200_quantize_rows_s8(const void* w, uint64_t ld_w, int8_t* q, uint64_t ld_q, float* scales, uint64_t n, uint64_t k,
                                                    const float* col_scale, void* stream);
 
+/* ---- activations in 8 bits -----------------------------------------------------------------------------------------------------
+ *
+ * int8 rows with ONE float32 scale a token, multiplied by the int8 weights of sepal_b200_gemm_w8r (one scale an output row) on the integer
+ * tensor pipe: the reference's W8A8 path (launch_gemm_s8 and the row quantiser, runner/cuda/src/gemm_s8_kernels.{cu,hpp}). A layer's MLP is
+ * sepal_b200_rms_norm_s8 -> sepal_b200_gemm_s8 (SWIGLU) -> sepal_b200_quantize_tokens_s8 -> sepal_b200_gemm_s8 (ADD). The three calls
+ * run on the context's device and allocate nothing. A token's bytes, scale and results depend on that token and the weights alone: not
+ * on the other rows of the call, and not on the schedule. */
+
+/* The residual's addition, the zero-centred RMSNorm and the token's quantisation in one pass:
+ *   x[t, :] += delta[t, :]   (delta NULL: nothing is added and x is only read; otherwise binary16 (delta_half != 0) or float32, one float32 addition)
+ *   v[t, c] = x[t, c] / sqrt(sum(x[t, :]^2) / cols + eps) * (1 + w[c]) * col_scale[c]   (col_scale NULL: 1; else the smoothing factors, cols floats)
+ *   scales[t] = max|v[t, :]| / 127,   q[t, c] = round to nearest even of v[t, c] * (127 / max|v[t, :]|)
+ * in float32 (the sum's order is not the reference kernel's). A token whose v is all zero gets scale 0 and zeros. One with a NaN or an
+ * infinity in v, or whose sum of squares overflows, gets scale NaN and zeros, so that its products are NaN; the other tokens do not see
+ * it. eps at least 1e-30. Any cols >= 1, strides and alignments; multiples of 4 values with 16-byte aligned x, w and col_scale rows are the fast form.
+ * Nothing outside the cols columns of a row is written. q may not overlap x, delta, w or col_scale. rows == 0 is a no-op. */
+SEPAL_B200_API int32_t sepal_b200_rms_norm_s8(sepal_b200_ctx* ctx, float* x, uint64_t ld_x, const void* delta, uint64_t ld_delta, int32_t delta_half,
+                                              const float* w, const float* col_scale, int8_t* q, uint64_t ld_q, float* scales, uint64_t rows,
+                                              uint64_t cols, float eps, void* stream);
+
+/* The quantisation alone (v = x * col_scale), for activations that no norm makes: a mixer's output, the SwiGLU's. x binary16 (x_half != 0)
+ * or float32 [rows, ld_x]. On binary16 rows the bits are those of sepal_b200_quantize_rows_s8. Multiples of 8 (binary16) or 4 values
+ * with 16-byte aligned x and col_scale rows are the fast form. */
+SEPAL_B200_API int32_t sepal_b200_quantize_tokens_s8(sepal_b200_ctx* ctx, const void* x, uint64_t ld_x, int32_t x_half, const float* col_scale, int8_t* q,
+                                                     uint64_t ld_q, float* scales, uint64_t rows, uint64_t cols, void* stream);
+
+/* Y[t, n] = epilogue( float32(sum over k of x[t, k] * w[n, k]) * sx[t] * sw[n] ): the sum an exact 32-bit integer (tcgen05.mma kind::i8), the
+ * scales multiplied in float32, the token's first; result binary16 (y_half != 0) or float32. x int8 [T, ld_x], sx [T]: what the two calls
+ * above leave; w int8 [N, ld_w], sw [N]: what sepal_b200_quantize_rows_s8 leaves. Epilogues as the other multiplies (a SWIGLU's w rows and
+ * sw in the packed order of sepal_b200_pack_gate_up). Requires 1 <= K < 131072, ld_x and ld_w multiples of 16, x and w 16-byte aligned;
+ * SWIGLU needs N a multiple of 128. Y of any alignment (16-byte aligned rows are the fast form). config: -1 chooses from the shape; 512 + w (w = 32, 64,
+ * ..., 256 tokens to a tile) forces the kernel on CTA pairs, 1024 + s or 1024 + 16 + s (s = 1 .. 8 parts of k; at most 128 rows, or 256 in the
+ * second form, with one CTA to an SM) the few-rows kernel. Every config gives the same bits. t == 0 is a no-op. */
+SEPAL_B200_API int32_t sepal_b200_gemm_s8(sepal_b200_ctx* ctx, const int8_t* x, uint64_t ld_x, const float* sx, const int8_t* w, uint64_t ld_w,
+                                          const float* sw, void* y, uint64_t ld_y, int32_t y_half, uint64_t t, uint64_t n, uint64_t k,
+                                          int32_t epilogue, int32_t config, void* stream);
+
 /* The group quantiser, bit for bit launch_quantize_group_s8 (runner/cuda/src/gemm_simt_kernels.hpp:64-65): src float32 [rows, K],
  * q int8 [rows, ld_q], s float32 [rows, ld_s] with one scale per group of 128. */
 SEPAL_B200_API int32_t sepal_b200_quantize_group_s8(const float* src, uint64_t ld_src, int8_t* q, uint64_t ld_q, float* s, uint64_t ld_s,

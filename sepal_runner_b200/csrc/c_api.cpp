@@ -16,8 +16,10 @@
 #include "checkpoint.hpp"
 #include "deltanet.hpp"
 #include "gemm.hpp"
+#include "gemm_s8.hpp"
 #include "model.hpp"
 #include "provider.hpp"
+#include "rows_s8.hpp"
 #include "trunk.hpp"
 
 using namespace sepal::b200;
@@ -92,7 +94,7 @@ int32_t sepal_b200_info(sepal_b200_ctx* ctx, char* buffer, uint64_t capacity, ui
                                  ",\"compute_capability\":\"" + std::to_string(c.compute_major) + "." + std::to_string(c.compute_minor) +
                                  "\",\"sm_count\":" + std::to_string(c.sm_count) + ",\"workspace_bytes\":" + std::to_string(c.scratch.partial_bytes) +
                                  ",\"kernels\":[\"gemm_tc_kernel<W8> (tcgen05.mma kind::f16, TMA, TMEM)\",\"gemm_pair_kernel\",\"gemm_w8_pair_kernel\",\"gemm_w8t_pair_kernel\","
-                                 "\"gemm_f16t_pair_kernel\",\"gemm_few_kernel\",\"quantize_group_s8_kernel\","
+                                 "\"gemm_f16t_pair_kernel\",\"gemm_few_kernel\",\"gemm_s8_pair_kernel\",\"gemm_s8_few_kernel\",\"rms_norm_s8_kernel\",\"quantize_tokens_s8_kernel\",\"quantize_group_s8_kernel\","
                                  "\"prepare_scales_kernel\",\"pack_gate_up_kernel\"],\"fallback\":\"none\"}";
         if (needed != nullptr) *needed = json.size() + 1;
         if (buffer == nullptr || capacity < json.size() + 1) throw std::length_error("buffer too small: " + std::to_string(json.size() + 1) + " bytes needed");
@@ -181,6 +183,30 @@ int32_t sepal_b200_gemm_w8r(sepal_b200_ctx* ctx, const void* x, uint64_t ld_x, c
 int32_t sepal_b200_quantize_rows_s8(const void* w, uint64_t ld_w, int8_t* q, uint64_t ld_q, float* scales, uint64_t n, uint64_t k, const float* col_scale,
                                     void* stream) {
     return guarded([&] { launch_quantize_rows_s8(w, ld_w, q, ld_q, scales, n, k, col_scale, static_cast<cudaStream_t>(stream)); });
+}
+
+int32_t sepal_b200_rms_norm_s8(sepal_b200_ctx* ctx, float* x, uint64_t ld_x, const void* delta, uint64_t ld_delta, int32_t delta_half, const float* w,
+                               const float* col_scale, int8_t* q, uint64_t ld_q, float* scales, uint64_t rows, uint64_t cols, float eps, void* stream) {
+    return guarded([&] {
+        require(ctx, "ctx");
+        launch_rms_norm_s8(ctx->ctx, x, ld_x, delta, ld_delta, delta_half != 0, w, col_scale, q, ld_q, scales, rows, cols, eps, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t sepal_b200_quantize_tokens_s8(sepal_b200_ctx* ctx, const void* x, uint64_t ld_x, int32_t x_half, const float* col_scale, int8_t* q, uint64_t ld_q,
+                                      float* scales, uint64_t rows, uint64_t cols, void* stream) {
+    return guarded([&] {
+        require(ctx, "ctx");
+        launch_quantize_tokens_s8(ctx->ctx, x, ld_x, x_half != 0, col_scale, q, ld_q, scales, rows, cols, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int32_t sepal_b200_gemm_s8(sepal_b200_ctx* ctx, const int8_t* x, uint64_t ld_x, const float* sx, const int8_t* w, uint64_t ld_w, const float* sw, void* y,
+                           uint64_t ld_y, int32_t y_half, uint64_t t, uint64_t n, uint64_t k, int32_t epilogue, int32_t config, void* stream) {
+    return guarded([&] {
+        require(ctx, "ctx");
+        launch_gemm_s8(ctx->ctx, x, ld_x, sx, w, ld_w, sw, y, ld_y, y_half != 0, t, n, k, epilogue_of(epilogue), config, static_cast<cudaStream_t>(stream));
+    });
 }
 
 int32_t sepal_b200_quantize_group_s8(const float* src, uint64_t ld_src, int8_t* q, uint64_t ld_q, float* s, uint64_t ld_s, uint64_t rows, uint64_t k,

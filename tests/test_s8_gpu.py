@@ -1,0 +1,465 @@
+"""Activations in 8 bits: the norm and the quantiser that leave int8 rows with a scale a token, and the int8 x int8 multiply, against the
+formulas in 64 bits.
+
+Tolerances. A byte is the rounding of u * 127 / max|u|: u carries at most three float32 roundings (1 + w, the two products), 127 / max one, their
+product one, max one of u's three: under 8 halves of a float32 step, so the byte is within 0.5 + 127 * 8 * 2^-24 of the exact quotient. A scale adds the
+sum of squares (under 40 additions in any chain, halved by the square root) and four roundings: 32 * 2^-24 relative. The multiply's sums are
+exact integers, and its two products by the scales can be repeated in float32 to the bit."""
+import ctypes as C
+
+import pytest
+import torch
+
+import sepal_runner_b200 as sb
+
+pytestmark = pytest.mark.gpu
+
+STEP = 2.0**-24
+BYTE = 0.5 + 127 * 8 * STEP
+SCALE = 32 * STEP
+
+
+def generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(gen, *shape, std=1.0):
+    return torch.randn(shape, generator=gen, device="cuda") * std
+
+
+def check_rows(q, scales, v):
+    """q and scales against the 64-bit rows v [T, C], all finite."""
+    top = v.abs().amax(1, keepdim=True)
+    assert torch.allclose(scales.double(), top[:, 0] / 127, rtol=SCALE, atol=2.0**-149)
+    quotient = torch.where(top > 0, v * 127 / top, 0.0)
+    assert ((q.double() - quotient).abs() <= BYTE).all()
+    assert q.abs().max() <= 127
+
+
+def guarded_rows(t, c, pad=16, offset=0):
+    """int8 rows of c values inside a buffer of 99s, and a check that nothing else of it was written."""
+    ld = (c + 15) // 16 * 16 + pad
+    buffer = torch.full((t + 2, ld), 99, dtype=torch.int8, device="cuda")
+    q = buffer[1 : t + 1, offset : offset + c]
+
+    def untouched():
+        mask = torch.ones_like(buffer, dtype=torch.bool)
+        mask[1 : t + 1, offset : offset + c] = False
+        assert (buffer[mask] == 99).all()
+
+    return q, untouched
+
+
+# widths: a lone vector, not whole warps, the served models' (1024 .. 4096), what 1024 threads hold to the value and one vector more, odd ones
+WIDTHS = [4, 132, 1024, 2560, 4096, 16384, 16388, 20000, 1, 7, 1023, 2563]
+
+
+@pytest.mark.parametrize("cols", WIDTHS)
+@pytest.mark.parametrize("delta", [None, torch.float16, torch.float32])
+def test_norm(ctx, cols, delta):
+    gen = generator(cols)
+    t = 5
+    x = randn(gen, t, cols, std=3.0)
+    x[1] *= 1e-3
+    w, smooth = randn(gen, cols, std=0.3), torch.exp(randn(gen, cols, std=0.5))
+    d = None if delta is None else randn(gen, t, cols).to(delta)
+    want_x = x if d is None else x + d.float()
+    for col_scale in (None, smooth):
+        stream = x.clone()
+        q, untouched = guarded_rows(t, cols)
+        scales = torch.full((t + 2,), 7.0, device="cuda")
+        ctx.rms_norm_s8(stream, w, q, scales[1 : t + 1], delta=d, col_scale=col_scale, eps=1e-6)
+        assert torch.equal(stream, want_x)
+        v = want_x.double()
+        v = v / (v.square().mean(1, keepdim=True) + 1e-6).sqrt() * (1 + w.double())
+        check_rows(q, scales[1 : t + 1], v if col_scale is None else v * smooth.double())
+        untouched()
+        assert scales[0] == 7 and scales[t + 1] == 7
+
+
+@pytest.mark.parametrize("cols", [8, 264, 3584, 9728, 12288, 32768, 32776, 40000, 1, 7, 1023, 2564])
+@pytest.mark.parametrize("half", [True, False])
+def test_quantiser(ctx, cols, half):
+    gen = generator(cols + 1)
+    t = 4
+    x = randn(gen, t, cols, std=2.0).to(torch.float16 if half else torch.float32)
+    smooth = torch.exp(randn(gen, cols, std=0.5))
+    for col_scale in (None, smooth):
+        q, untouched = guarded_rows(t, cols)
+        _, scales = ctx.quantize_tokens_s8(x, q, col_scale=col_scale)
+        check_rows(q, scales, x.double() if col_scale is None else x.double() * smooth.double())
+        untouched()
+        if half and cols % 16 == 0:
+            # the weights' quantiser makes the same bytes and scales
+            want, want_scales = ctx.quantize_rows_s8(x, col_scale)
+            assert torch.equal(q, want) and torch.equal(scales, want_scales)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("ld", [2560, 2561, 2564, 2576])
+def test_alignments_do_not_change_the_bytes(ctx, offset, ld):
+    """Every base and stride gives the bytes and scales of contiguous rows, but the norm's scales, whose sum the two forms add in
+    different orders."""
+    gen = generator(ld + offset)
+    t, cols = 3, 2560 - 16
+    wide = randn(gen, t + 1, ld)
+    x = wide.flatten()[offset : offset + t * ld].view(t, ld)[:, :cols]
+    w = randn(gen, cols + 8, std=0.3)[offset % 5 : offset % 5 + cols]
+    delta = randn(gen, t, ld)[:, :cols]
+    q0, s0 = ctx.rms_norm_s8(x.contiguous(), w.clone(), delta=delta.contiguous())
+    q, untouched = guarded_rows(t, cols, offset=offset)
+    before = wide.clone()
+    _, s = ctx.rms_norm_s8(x, w, q, delta=delta)
+    assert torch.equal(q, q0) and torch.allclose(s, s0, rtol=2 * SCALE, atol=0)
+    untouched()
+    after = before.flatten().clone()
+    after[offset : offset + t * ld].view(t, ld)[:, :cols] += delta
+    assert torch.equal(wide.flatten(), after)  # the columns between the rows are as they were
+    for kind in (torch.float16, torch.float32):
+        xk = wide.to(kind).flatten()[offset : offset + t * ld].view(t, ld)[:, :cols]
+        q0, s0 = ctx.quantize_tokens_s8(xk.contiguous())
+        q, untouched = guarded_rows(t, cols, offset=offset)
+        _, s = ctx.quantize_tokens_s8(xk, q)
+        assert torch.equal(q, q0) and torch.equal(s, s0)
+        untouched()
+
+
+@pytest.mark.parametrize("cols", [256, 255])
+def test_rows_that_are_zero_tiny_huge_or_not_finite(ctx, cols):
+    """Each special row beside ordinary ones, whose bytes do not change."""
+    gen = generator(9)
+    x = randn(gen, 10, cols)
+    plain_q, plain_s = ctx.quantize_tokens_s8(x)
+    inf, nan = float("inf"), float("nan")
+    x[1] = 0
+    x[2] *= 1e-37          # 127 / max overflows without the lift
+    x[3] *= 1e-44          # float32's smallest numbers
+    x[4] *= 1e37 / x[4].abs().max()
+    x[5, 3] = nan
+    x[6, cols - 1] = inf
+    x[7, 0] = -inf
+    x[8, 5], x[8, 6] = inf, nan
+    w = torch.zeros(cols, device="cuda")
+    q, s = ctx.quantize_tokens_s8(x)
+    for r in (0, 9):
+        assert torch.equal(q[r], plain_q[r]) and s[r] == plain_s[r]
+    check_rows(q[1:5], s[1:5], x[1:5].double())
+    assert s[1] == 0 and (q[1] == 0).all()
+    assert torch.isnan(s[5:9]).all() and (q[5:9] == 0).all()
+    qn, sn = ctx.rms_norm_s8(x, w)
+    v = x[:4].double()
+    check_rows(qn[:4], sn[:4], v / (v.square().mean(1, keepdim=True) + 1e-6).sqrt())
+    # squares beyond float32, and what is not finite: NaN and zeros
+    assert torch.isnan(sn[4:9]).all() and (qn[4:9] == 0).all()
+    # what the gains make infinite
+    q2, s2 = ctx.rms_norm_s8(x[:1] * 10, torch.full((cols,), 3e38, device="cuda"))
+    assert torch.isnan(s2).all() and (q2 == 0).all()
+    # the binary16 type's own ends
+    h = torch.tensor([[65504.0, -65504.0, 1.0, 0.0], [5.96e-8, 0, 0, -5.96e-8]], device="cuda").half()
+    qh, sh = ctx.quantize_tokens_s8(h)
+    check_rows(qh, sh, h.double())
+
+
+def test_ties_go_to_even(ctx):
+    x = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -126.5, 125.5]], device="cuda")
+    for kind in (torch.float16, torch.float32):
+        q, s = ctx.quantize_tokens_s8(x.to(kind))
+        assert q.tolist() == [[127, 0, 2, 2, 0, -2, -126, 126]] and s.item() == 1.0
+
+
+def product(x, wq, sx, sw):
+    """The multiply's float32 result before its epilogue, to the bit: exact sums (64-bit floats hold them), rounded once, times the token's scale, times the row's."""
+    acc = x.double() @ wq.double().T
+    return acc.float() * sx[:, None] * sw
+
+
+def swiglu64(v):
+    b = v.double().view(v.shape[0], -1, 2, 64)
+    g, u = b[:, :, 0], b[:, :, 1]
+    value = g * torch.sigmoid(g) * u
+    # the exponential's documented error is 2 + 1.173 |g| steps of 2^-23, the quotient's two, the sum's and the product's one each
+    slack = value.abs() * (8 + 1.2 * g.abs()) * 2.0**-23 + 1e-30 * u.abs()
+    return value.reshape(v.shape[0], -1), slack.reshape(v.shape[0], -1)
+
+
+def operands(seed, t, n, k):
+    gen = generator(seed)
+    # rows of a buffer whose stride is more than the row, and not a multiple of 128
+    x = torch.randint(-127, 128, (t, (k + 15) // 16 * 16 + 16), generator=gen, device="cuda", dtype=torch.int8)[:, :k]
+    w = torch.randint(-127, 128, (n, (k + 15) // 16 * 16 + 48), generator=gen, device="cuda", dtype=torch.int8)[:, :k]
+    sx = torch.rand(t, generator=gen, device="cuda") * 0.05 + 0.001
+    sw = (torch.rand(n, generator=gen, device="cuda") + 0.1) * 0.02 / (k**0.5)
+    return gen, x, sx, w, sw
+
+
+def guarded_out(t, n, dtype, aligned=True):
+    size = 4 if dtype == torch.float32 else 2
+    step = 16 // size
+    ld = (n + step - 1) // step * step + step + (0 if aligned else 1)
+    buffer = torch.full((t + 2, ld), -77.0, dtype=dtype, device="cuda")
+    y = buffer[1 : t + 1, :n]
+    if not aligned:
+        y = buffer[1 : t + 1, 1 : n + 1]
+
+    def untouched():
+        mask = torch.ones_like(buffer, dtype=torch.bool)
+        mask[1 : t + 1, (0 if aligned else 1) : n + (0 if aligned else 1)] = False
+        assert (buffer[mask] == -77).all()
+
+    return y, untouched
+
+
+def check_multiply(ctx, t, n, k, configs, seed=3):
+    gen, x, sx, w, sw = operands(seed, t, n, k)
+    want = product(x, w, sx, sw)
+    old = randn(gen, t, n)
+    for config in configs:
+        for aligned in (True, False):
+            for dtype in (torch.float32, torch.float16):
+                y, untouched = guarded_out(t, n, dtype, aligned)
+                ctx.gemm_s8(x, sx, w, sw, y, config=config)
+                assert torch.equal(y, want.to(dtype)), (config, aligned, dtype)
+                untouched()
+                y, untouched = guarded_out(t, n, dtype, aligned)
+                y.copy_(old)
+                ctx.gemm_s8(x, sx, w, sw, y, epilogue=sb.ADD, config=config)
+                assert torch.equal(y, (old.to(dtype).float() + want).to(dtype)), (config, aligned, dtype)
+                untouched()
+                if n % 128 == 0:
+                    value, slack = swiglu64(want)
+                    y, untouched = guarded_out(t, n // 2, dtype, aligned)
+                    ctx.gemm_s8(x, sx, w, sw, y, epilogue=sb.SWIGLU, config=config)
+                    if dtype == torch.float16:
+                        slack = slack + value.abs() * 2.0**-11 + 2.0**-25
+                    assert ((y.double() - value).abs() <= slack).all(), (config, aligned, dtype)
+                    untouched()
+    ctx.check_status()
+
+
+# (1: lengths under a swizzled row, a step, the ring's depth and odd ones; tokens around a block; weight rows around a tile)
+@pytest.mark.parametrize("t,n,k", [(1, 1, 1), (1, 2, 16), (2, 130, 127), (15, 128, 129), (16, 256, 1360), (17, 1000, 1360), (64, 384, 2560), (65, 127, 640),
+                                   (128, 640, 1023), (129, 128, 2048), (256, 257, 384)])
+def test_multiply_few_rows(ctx, t, n, k):
+    check_multiply(ctx, t, n, k, [-1] + [1024 + s for s in (1, 2, 3, 5, 8) if t <= 128] + [1024 + 16 + s for s in (1, 4, 7)])
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 1, 1), (31, 255, 100), (33, 256, 128), (129, 384, 1360), (200, 1000, 640), (257, 130, 2560), (130, 252, 256), (130, 264, 256), (300, 512, 1024), (777, 640, 4096)])
+def test_multiply_on_pairs(ctx, t, n, k):
+    check_multiply(ctx, t, n, k, [-1, 512 + 32, 512 + 96, 512 + 160, 512 + 192, 512 + 256])
+
+
+def test_multiply_many_tiles_to_a_pair(ctx):
+    """More tiles than CTA pairs: the two accumulators and the ring go round many times."""
+    check_multiply(ctx, 1500, 2560, 384, [-1, 512 + 64, 512 + 256])
+
+
+@pytest.mark.parametrize("t,n,k,epilogue,dtype", [(900, 2560, 9728, sb.ADD, torch.float32), (4096, 2560, 2048, sb.ADD, torch.float32), (1337, 6144, 2560, sb.STORE, torch.float16),
+                                                  (1, 6144, 2560, sb.STORE, torch.float16), (29, 2560, 9728, sb.ADD, torch.float32), (200, 1024, 3584, sb.ADD, torch.float32)])
+def test_multiply_at_the_models_sizes(ctx, t, n, k, epilogue, dtype):
+    gen, x, sx, w, sw = operands(t, t, n, k)
+    want = product(x, w, sx, sw)
+    y = randn(gen, t, n).to(dtype)
+    if epilogue == sb.ADD:
+        want = want + y
+    ctx.gemm_s8(x, sx, w, sw, y, epilogue=epilogue)
+    ctx.check_status()
+    assert torch.equal(y, want.to(dtype))
+
+
+def test_the_largest_sums_fit(ctx):
+    """131071 products of -128 * -128 are the largest sum that 32 bits hold."""
+    k = (1 << 17) - 1
+    x = torch.full((3, k + 1), -128, dtype=torch.int8, device="cuda")[:, :k]
+    w = torch.full((16, k + 1), -128, dtype=torch.int8, device="cuda")[:, :k]
+    w[1] = 127
+    one = torch.ones(16, device="cuda")
+    for config in (-1, 1024 + 8, 512 + 32):
+        y = ctx.gemm_s8(x, one[:3], w, one, y_half=False, config=config)
+        ctx.check_status()
+        assert (y[:, 0] == float(128 * 128 * k)).all() and (y[:, 1] == float(-128 * 127 * k)).all() and torch.equal(y[:, 2:], y[:, :1].expand(3, 14))
+
+
+def test_scales_that_are_not_finite_stay_in_their_row_and_column(ctx):
+    gen, x, sx, w, sw = operands(8, 70, 256, 512)
+    want = product(x, w, sx, sw)
+    sx[3], sx[65] = float("nan"), 0.0
+    sw[7] = float("inf")
+    x[4] = 0
+    for config in (1024 + 2, 512 + 64):
+        y = ctx.gemm_s8(x, sx, w, sw, y_half=False, config=config)
+        ctx.check_status()
+        assert torch.isnan(y[3]).all()
+        assert (y[65, :7] == 0).all() and torch.isnan(y[65, 7]) and torch.isnan(y[4, 7])
+        keep = torch.ones(70, 256, dtype=torch.bool, device="cuda")
+        keep[[3, 4, 65]] = False
+        keep[:, 7] = False
+        assert torch.equal(y[keep], want[keep])
+
+
+def test_a_row_does_not_depend_on_the_others(ctx):
+    """One token alone, in a few and among many: the same bytes, scale and products."""
+    gen, _, _, w, sw = operands(21, 1, 384, 1024)
+    x, g = randn(gen, 700, 1024, std=2.0), randn(gen, 1024, std=0.3)
+    q, s = ctx.rms_norm_s8(x, g)
+    y = ctx.gemm_s8(q, s, w, sw, y_half=False)
+    for first, count in ((0, 1), (699, 1), (17, 30), (100, 200)):
+        q1, s1 = ctx.rms_norm_s8(x[first : first + count], g)
+        assert torch.equal(q1, q[first : first + count]) and torch.equal(s1, s[first : first + count])
+        assert torch.equal(ctx.gemm_s8(q1, s1, w, sw, y_half=False), y[first : first + count])
+    ctx.check_status()
+
+
+def test_nothing_to_do(ctx):
+    w = torch.zeros(64, device="cuda")
+    q, s = ctx.rms_norm_s8(torch.zeros((0, 64), device="cuda"), w)
+    assert q.shape == (0, 64) and s.shape == (0,)
+    q, s = ctx.quantize_tokens_s8(torch.zeros((0, 64), device="cuda").half())
+    assert q.shape == (0, 64)
+    y = ctx.gemm_s8(q, s, torch.zeros((8, 64), dtype=torch.int8, device="cuda"), w[:8])
+    assert y.shape == (0, 8)
+    ctx.check_status()
+
+
+def mlp(ctx, x, delta, norm_w, gate_up, gate_up_s, down, down_s, buffers):
+    """A layer's second half as an engine runs it: norm, gate and up, SwiGLU, down, onto the stream."""
+    q, s, a, aq, as_ = buffers
+    ctx.rms_norm_s8(x, norm_w, q, s, delta=delta)
+    ctx.gemm_s8(q, s, gate_up, gate_up_s, a, epilogue=sb.SWIGLU)
+    ctx.quantize_tokens_s8(a, aq, as_)
+    ctx.gemm_s8(aq, as_, down, down_s, x, epilogue=sb.ADD)
+
+
+def mlp_operands(ctx, t, hidden, inner, seed):
+    gen = generator(seed)
+    x, delta, norm_w = randn(gen, t, hidden, std=2.0), randn(gen, t, hidden).half(), randn(gen, hidden, std=0.2)
+    stacked = randn(gen, 2 * inner, hidden, std=0.02).half()
+    gate_up, gate_up_s = ctx.quantize_rows_s8(ctx.pack_gate_up(stacked))
+    down, down_s = ctx.quantize_rows_s8(randn(gen, hidden, inner, std=0.02).half())
+    empty = lambda *shape, dtype: torch.empty(shape, dtype=dtype, device="cuda")  # noqa: E731
+    buffers = (empty(t, hidden, dtype=torch.int8), empty(t, dtype=torch.float32), empty(t, inner, dtype=torch.float16), empty(t, inner, dtype=torch.int8), empty(t, dtype=torch.float32))
+    return x, delta, norm_w, stacked, gate_up, gate_up_s, down, down_s, buffers
+
+
+@pytest.mark.parametrize("t", [1, 29, 300])
+def test_a_layers_mlp(ctx, t):
+    """The calls together, each step held to its formula on what the step before left in the engine's buffers."""
+    hidden, inner = 1024, 1792
+    x, delta, norm_w, _, gate_up, gate_up_s, down, down_s, buffers = mlp_operands(ctx, t, hidden, inner, 5 + t)
+    start = x.clone()
+    mlp(ctx, x, delta, norm_w, gate_up, gate_up_s, down, down_s, buffers)
+    ctx.check_status()
+    q, s, a, aq, as_ = buffers
+    stream = start + delta.float()
+    v = stream.double()
+    check_rows(q, s, v / (v.square().mean(1, keepdim=True) + 1e-6).sqrt() * (1 + norm_w.double()))
+    value, slack = swiglu64(product(q, gate_up, s, gate_up_s))
+    assert ((a.double() - value).abs() <= slack + value.abs() * 2.0**-11 + 2.0**-25).all()
+    check_rows(aq, as_, a.double())
+    assert torch.equal(x, stream + product(aq, down, as_, down_s))
+
+
+def test_a_captured_mlp_replays_on_new_inputs(ctx):
+    """Captured once, replayed over other inputs in the same buffers: the eager calls' bits."""
+    t, hidden, inner = 65, 512, 640
+    own = sb.Context(0)
+    x, delta, norm_w, _, gate_up, gate_up_s, down, down_s, buffers = mlp_operands(own, t, hidden, inner, 2)
+    first = x.clone()
+    mlp(own, x, delta, norm_w, gate_up, gate_up_s, down, down_s, buffers)
+    eager = x.clone()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        mlp(own, x, delta, norm_w, gate_up, gate_up_s, down, down_s, buffers)
+    other = randn(generator(77), t, hidden)
+    for source in (first, other, first):
+        x.copy_(source)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = x.clone()
+        x.copy_(source)
+        mlp(own, x, delta, norm_w, gate_up, gate_up_s, down, down_s, buffers)
+        assert torch.equal(got, x)
+        if source is first:
+            assert torch.equal(got, eager)
+    own.check_status()
+    del graph
+    own.close()
+
+
+def test_two_streams_with_a_context_each():
+    """Two engines on one GPU: each its own context and stream, the calls in flight together."""
+    contexts, streams = [sb.Context(0), sb.Context(0)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    work = [mlp_operands(c, t, 512, 640, 30 + t) for c, t in zip(contexts, (40, 333))]
+    alone = []
+    for c, (x, delta, norm_w, _, gu, gus, dn, dns, buffers) in zip(contexts, work):
+        start = x.clone()
+        mlp(c, x, delta, norm_w, gu, gus, dn, dns, buffers)
+        alone.append(x.clone())
+        x.copy_(start)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        starts = [w[0].clone() for w in work]
+        torch.cuda.synchronize()
+        for c, s, (x, delta, norm_w, _, gu, gus, dn, dns, buffers) in zip(contexts, streams, work):
+            with torch.cuda.stream(s):
+                mlp(c, x, delta, norm_w, gu, gus, dn, dns, buffers)
+        torch.cuda.synchronize()
+        for (x, *_), want, start in zip(work, alone, starts):
+            assert torch.equal(x, want)
+            x.copy_(start)
+        torch.cuda.synchronize()
+    for c in contexts:
+        c.check_status()
+        c.close()
+
+
+def test_launch_overlap_and_static_weights_change_no_bits():
+    """Back to back on one stream, as dependents and in plain order, with and without the promise of static weights."""
+    results = []
+    for overlap in (True, False):
+        for static in (False, True):
+            sb.library().sepal_b200_set_launch_overlap(1 if overlap else 0)
+            c = sb.Context(0)
+            c.set_static_weights(static)
+            x, delta, norm_w, _, gu, gus, dn, dns, buffers = mlp_operands(c, 200, 512, 640, 4)
+            torch.cuda.synchronize()
+            for _ in range(8):
+                mlp(c, x, delta, norm_w, gu, gus, dn, dns, buffers)
+            c.check_status()
+            results.append(x)
+            c.close()
+    sb.library().sepal_b200_set_launch_overlap(1)
+    assert all(torch.equal(r, results[0]) for r in results[1:])
+
+
+def test_refusals_of_the_library(ctx):
+    """What the C ABI refuses, with a message and before anything is launched."""
+    lib, h = ctx._lib, ctx._h
+    x = torch.zeros((4, 64), device="cuda")
+    q = torch.zeros((4, 64), dtype=torch.int8, device="cuda")
+    s, y = torch.zeros(64, device="cuda"), torch.full((4, 128), 5.0, device="cuda")
+
+    def norm(ld_x=64, delta=None, ld_delta=64, w=s, ld_q=64, cols=64, eps=1e-6, rows=4):
+        return lib.sepal_b200_rms_norm_s8(h, x.data_ptr(), ld_x, delta, ld_delta, 0, None if w is None else w.data_ptr(), None, q.data_ptr(), ld_q, s.data_ptr(), rows, cols,
+                                          eps, None)
+
+    def multiply(xq=None, ld_x=64, ld_w=64, ld_y=64, n=64, k=64, epilogue=0, config=-1, t=4, sx=s):
+        return lib.sepal_b200_gemm_s8(h, q.data_ptr() if xq is None else xq, ld_x, None if sx is None else sx.data_ptr(), q.data_ptr(), ld_w, s.data_ptr(), y.data_ptr(),
+                                      ld_y, 0, t, n, k, epilogue, config, None)
+
+    for call in (lambda: norm(ld_x=63), lambda: norm(ld_q=63), lambda: norm(delta=x.data_ptr(), ld_delta=63), lambda: norm(w=None), lambda: norm(cols=0),
+                 lambda: norm(eps=0.0), lambda: norm(eps=-1.0), lambda: norm(eps=float("nan")), lambda: norm(eps=float("inf")), lambda: norm(rows=1 << 31),
+                 lambda: multiply(ld_x=72), lambda: multiply(ld_x=48), lambda: multiply(ld_w=72), lambda: multiply(ld_y=63), lambda: multiply(k=0),
+                 lambda: multiply(n=0), lambda: multiply(k=1 << 17, ld_x=1 << 17, ld_w=1 << 17), lambda: multiply(epilogue=2), lambda: multiply(epilogue=3),
+                 lambda: multiply(xq=q.data_ptr() + 8), lambda: multiply(sx=None), lambda: multiply(config=0), lambda: multiply(config=-2), lambda: multiply(config=512),
+                 lambda: multiply(config=512 + 33), lambda: multiply(config=512 + 288), lambda: multiply(config=1024), lambda: multiply(config=1024 + 9),
+                 lambda: multiply(config=1024 + 25), lambda: multiply(config=2048), lambda: multiply(config=1024 + 2, t=129), lambda: multiply(config=1024 + 18, t=257)):
+        assert call() != 0
+        assert len(lib.sepal_b200_last_error()) > 10
+    out = C.c_int32(0)
+    assert lib.sepal_b200_status(h, None, C.byref(out)) == 0 and out.value == 0
+    assert (y == 5).all() and (q == 0).all()
+    # nothing to do is no error, whatever the pointers
+    assert lib.sepal_b200_rms_norm_s8(h, None, 64, None, 0, 0, None, None, None, 64, None, 0, 64, 1e-6, None) == 0
+    assert lib.sepal_b200_quantize_tokens_s8(h, None, 64, 1, None, None, 64, None, 0, 64, None) == 0
+    assert lib.sepal_b200_gemm_s8(h, None, 64, None, None, 64, None, None, 64, 0, 0, 64, 64, 0, -1, None) == 0

@@ -1,0 +1,86 @@
+"""What the 8-bit activation calls refuse before they touch a device: through the binding (shapes, types, devices) and through the C ABI."""
+import types
+
+import pytest
+import torch
+
+import sepal_runner_b200 as sb
+from sepal_runner_b200 import lib as sbl
+
+
+@pytest.fixture()
+def bare():
+    """A Context without a device behind it, whose C calls fail the test: every call here must be refused before one."""
+    c = sb.Context.__new__(sb.Context)
+
+    def called(*_):
+        raise AssertionError("a refused call reached the library")
+
+    c._lib = types.SimpleNamespace(sepal_b200_rms_norm_s8=called, sepal_b200_quantize_tokens_s8=called, sepal_b200_gemm_s8=called)
+    c._h, c.device = None, 0
+    return c
+
+
+def test_tensors_of_another_device_are_refused(bare):
+    with pytest.raises(ValueError, match="cuda:0"):
+        bare.rms_norm_s8(torch.zeros(4, 64), torch.zeros(64))
+    with pytest.raises(ValueError, match="cuda:0"):
+        bare.quantize_tokens_s8(torch.zeros(4, 64))
+    with pytest.raises(ValueError, match="cuda:0"):
+        bare.gemm_s8(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4), torch.zeros(8, 64, dtype=torch.int8), torch.ones(8))
+
+
+def test_shapes_types_and_strides_are_refused(bare, monkeypatch):
+    # the device test is the one thing that CPU tensors cannot pass
+    monkeypatch.setattr(sbl, "_rows_of", lambda t, device: t.numel() == 0 or t.stride(-1) == 1)
+    x, w = torch.zeros(4, 64), torch.zeros(64)
+    for bad in (x.double(), x.half(), x[0], x.t()):
+        with pytest.raises(ValueError, match="x must be"):
+            bare.rms_norm_s8(bad, w)
+    with pytest.raises(ValueError, match="w must be"):
+        bare.rms_norm_s8(x, w)  # (on the CPU)
+    monkeypatch.setattr(sbl, "_require_floats", lambda t, n, device, who, what: None if t.numel() == n and t.dtype == torch.float32 else (_ for _ in ()).throw(ValueError(f"{what} must be")))
+    for bad in (torch.zeros(63), torch.zeros(64).half()):
+        with pytest.raises(ValueError, match="w must be"):
+            bare.rms_norm_s8(x, bad)
+        with pytest.raises(ValueError, match="col_scale must be"):
+            bare.rms_norm_s8(x, w, col_scale=bad)
+        with pytest.raises(ValueError, match="col_scale must be"):
+            bare.quantize_tokens_s8(x, col_scale=bad)
+    for bad in (torch.zeros(4, 63), torch.zeros(3, 64), torch.zeros(4, 64).bfloat16()):
+        with pytest.raises(ValueError, match="delta must be"):
+            bare.rms_norm_s8(x, w, delta=bad)
+    with pytest.raises(ValueError, match="overlap"):
+        bare.rms_norm_s8(torch.zeros(64).expand(4, 64), w, delta=x)
+    for bad in (torch.zeros(4, 64), torch.zeros(4, 48, dtype=torch.int8), torch.zeros(64, 4, dtype=torch.int8).t()):
+        with pytest.raises(ValueError, match="q must be"):
+            bare.rms_norm_s8(x, w, bad, torch.zeros(4))
+    for bad in (x.double(), x.bfloat16(), x[0], x.t()):
+        with pytest.raises(ValueError, match="x must be"):
+            bare.quantize_tokens_s8(bad)
+    xq, wq, sx, sw = torch.zeros(4, 64, dtype=torch.int8), torch.zeros(8, 64, dtype=torch.int8), torch.ones(4), torch.ones(8)
+    for a, b in ((xq.float(), wq), (xq, wq.half()), (xq[0], wq), (xq.t(), wq), (xq, wq.t())):
+        with pytest.raises(ValueError, match="int8 matrices"):
+            bare.gemm_s8(a, sx, b, sw)
+    with pytest.raises(ValueError, match="inner dimensions"):
+        bare.gemm_s8(xq, sx, wq[:, :48], sw)
+    with pytest.raises(ValueError, match="sx must be"):
+        bare.gemm_s8(xq, sx[:3], wq, sw)
+    with pytest.raises(ValueError, match="sw must be"):
+        bare.gemm_s8(xq, sx, wq, sw.half())
+    with pytest.raises(ValueError, match="ADD"):
+        bare.gemm_s8(xq, sx, wq, sw, epilogue=sb.ADD)
+    with pytest.raises(ValueError, match="output must be"):
+        bare.gemm_s8(xq, sx, wq, sw, torch.zeros(4, 9))
+    with pytest.raises(ValueError, match="float16 or float32"):
+        bare.gemm_s8(xq, sx, wq, sw, torch.zeros(4, 8).bfloat16())
+
+
+def test_no_context_is_an_error_and_not_a_crash():
+    lib = sb.library()
+    assert lib.sepal_b200_rms_norm_s8(None, None, 4, None, 0, 0, None, None, None, 4, None, 1, 4, 1e-6, None) != 0
+    assert b"ctx is null" in lib.sepal_b200_last_error()
+    assert lib.sepal_b200_quantize_tokens_s8(None, None, 4, 1, None, None, 4, None, 1, 4, None) != 0
+    assert b"ctx is null" in lib.sepal_b200_last_error()
+    assert lib.sepal_b200_gemm_s8(None, None, 16, None, None, 16, None, None, 8, 1, 1, 8, 16, 0, -1, None) != 0
+    assert b"ctx is null" in lib.sepal_b200_last_error()
