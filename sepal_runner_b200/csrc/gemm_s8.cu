@@ -60,12 +60,46 @@ __device__ __forceinline__ float scaled(int sum, float sx, float sw) { return __
 //               column, its registers run along the tokens; a chunk leaves transposed through the warp's staging boxes and the TMA (a store,
 //               or a reduce-add for the float32 residual update), or lane by lane where Y's rows are not 16-byte aligned.
 constexpr unsigned kPairThreads = 320;
-constexpr unsigned kMaxStages = 8;
+constexpr unsigned kMaxStages = 12;
 constexpr unsigned kAccStride = 256;          // tensor-memory columns from one accumulator to the other
 constexpr unsigned kEpilogueWarps = 8;
 constexpr unsigned kBoxBytes = 2048;          // a staging box: 16 tokens x 32 float32, or 32 x 32 binary16; two to a warp
 constexpr unsigned kPairBarriers = 2 * kMaxStages + 4;
 constexpr unsigned kPairTail = kEpilogueWarps * 128 + kPairBarriers * 8 + 64;
+
+// The issuing roles are run by a whole warp, every branch but the elected thread's own the same for all of it. Addresses and descriptors then
+// stay in the warp's uniform registers, which the asynchronous instructions take their operands from; in a loop run by one thread (if
+// lane == 0) each is moved there for every instruction: 468 clocks a step of four MMAs where the tensor cores need 2 bt.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(one));
+    return one != 0;
+}
+// wait_barrier by a whole warp: every branch is the same for all of it, so that the loops around it stay in uniform registers.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile unsigned* abort_flag, int* status, int code) {
+    if (__all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(bar, parity))) return true;
+    const long long t0 = clock64();
+    for (unsigned spins = 1;; ++spins) {
+        if (__all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(bar, parity))) return true;
+        if ((spins & 31u) == 0) {
+            const bool late = clock64() - t0 > kWaitLimit;
+            if (__any_sync(0xFFFFFFFFu, late || *abort_flag != 0)) {
+                if (__any_sync(0xFFFFFFFFu, late) && threadIdx.x % 32 == 0) {
+                    *abort_flag = 1;
+                    atomicCAS(status, 0, code | (static_cast<int>(blockIdx.x) << 8));
+                }
+                __syncwarp();
+                return false;
+            }
+        }
+    }
+}
 
 // Both warps that share a chunk of the SwiGLU arrive with their own `ok`; true when both are.
 __device__ __forceinline__ bool both_agree(uint32_t id, bool ok) {
@@ -120,7 +154,7 @@ gemm_s8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     unsigned* const words = reinterpret_cast<unsigned*>(tail + kEpilogueWarps * 128 + kPairBarriers * 8);
     volatile unsigned* const abort_flag = words + 1;
 
-    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const unsigned warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // (the shuffle: known to be the same in the warp)
     const unsigned rank = ptx::cluster_ctarank();
     const unsigned pair = blockIdx.x / 2, pairs = gridDim.x / 2;
 
@@ -146,85 +180,94 @@ gemm_s8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     __syncthreads();
     ptx::cluster_sync();  // the partner's barriers exist before anything signals them
     ptx::tc_fence_after_sync();
-    const uint32_t tmem_base = words[0];
+    const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, words[0], 0);
     ptx::grid_launch_dependents();
     // Static weights: the first tiles of W are requested before the kernel before this one has finished.
-    unsigned early = 0;
-    if (p.early_w != 0 && threadIdx.x == 0) {
-        early = min(p.stages, p.k_iters);
+    const uint32_t full0 = ptx::map_to_cta(full_bar(0), 0);  // a step's bytes are counted in the first CTA
+    const unsigned early = p.early_w != 0 ? min(p.stages, p.k_iters) : 0u;
+    if (warp == 0 && early != 0) {
+        const bool one = elect_one();
         const int row_w = static_cast<int>(pair / p.t_tiles * 256 + rank * kRows);
         for (unsigned i = 0; i < early; ++i) {
-            if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(i), 2 * stage_bytes);
-            ptx::tma_load_2d_pair(base + i * stage_bytes, &map_w, ptx::map_to_cta(full_bar(i), 0), static_cast<int>(i * kBK), row_w);
+            if (one) {
+                if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(i), 2 * stage_bytes);
+                ptx::tma_load_2d_pair(base + i * stage_bytes, &map_w, full0 + 8u * i, static_cast<int>(i * kBK), row_w);
+            }
         }
+        __syncwarp();
     }
     ptx::grid_dependency_wait();
 
     // tile = weight tile * t_tiles + token tile, dealt round-robin: the pairs of a wave share few weight tiles and most of X, which the L2 holds
     if (warp == 0) {
-        if (lane == 0) {
-            int stage = 0;
-            unsigned phase = 0, issued = 0;
-            bool ok = true;
-            for (unsigned tile = pair; ok && tile < p.tiles; tile += pairs) {
-                const int row_w = static_cast<int>(tile / p.t_tiles * 256 + rank * kRows);
-                const int row_x = static_cast<int>(tile % p.t_tiles * bt + rank * (bt / 2));
-                for (unsigned i = 0; i < p.k_iters; ++i, ++issued) {
-                    const bool begun = issued < early;
-                    if (!begun && !wait_barrier(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kStatusProducerEmpty)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t dst = base + stage * stage_bytes;
-                    const uint32_t full_first = ptx::map_to_cta(full_bar(stage), 0);
+        const bool one = elect_one();
+        int stage = 0;
+        unsigned phase = 0, issued = 0;
+        bool ok = true;
+        for (unsigned tile = pair; ok && tile < p.tiles; tile += pairs) {
+            const int row_w = static_cast<int>(tile / p.t_tiles * 256 + rank * kRows);
+            const int row_x = static_cast<int>(tile % p.t_tiles * bt + rank * (bt / 2));
+            for (unsigned i = 0; i < p.k_iters; ++i, ++issued) {
+                const bool begun = issued < early;
+                if (!begun && !wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kStatusProducerEmpty)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t dst = base + stage * stage_bytes, bar = full_bar(stage), full_first = full0 + 8u * stage;
+                if (one) {
                     if (!begun) {
-                        if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * stage_bytes);
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(bar, 2 * stage_bytes);
                         ptx::tma_load_2d_pair(dst, &map_w, full_first, static_cast<int>(i * kBK), row_w);
                     }
                     ptx::tma_load_2d_pair(dst + kWBytes, &map_x, full_first, static_cast<int>(i * kBK), row_x);
-                    if (++stage == stages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                }
+                __syncwarp();
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            if (!ok) grace_for_copies_in_flight();
         }
-        __syncwarp();
+        if (!ok) grace_for_copies_in_flight();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const bool one = elect_one();
             const uint32_t idesc = ptx::instr_desc_s8_s32acc(256, bt);
+            const uint64_t dw0 = ptx::smem_desc_k_major_sw128(base), dx0 = ptx::smem_desc_k_major_sw128(base + kWBytes);
+            const uint32_t step16 = stage_bytes >> 4;
             int stage = 0, acc = 0;
             unsigned phase = 0, acc_phase = 0;
             bool ok = true;
             for (unsigned tile = pair; ok && tile < p.tiles; tile += pairs) {
-                if (!wait_barrier(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.status, kStatusMmaAccEmpty)) break;
+                if (!wait_warp(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, p.status, kStatusMmaAccEmpty)) break;
                 ptx::tc_fence_after_sync();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc) * kAccStride;
                 for (unsigned i = 0; i < p.k_iters; ++i) {
-                    if (!wait_barrier(full_bar(stage), phase, abort_flag, p.status, kStatusMmaFull)) {
+                    if (!wait_warp(full_bar(stage), phase, abort_flag, p.status, kStatusMmaFull)) {
                         ok = false;
                         break;
                     }
                     ptx::tc_fence_after_sync();
-                    const uint64_t dw = ptx::smem_desc_k_major_sw128(base + stage * stage_bytes);
-                    const uint64_t dx = ptx::smem_desc_k_major_sw128(base + stage * stage_bytes + kWBytes);
+                    const uint64_t dw = dw0 + stage * step16, dx = dx0 + stage * step16;
+                    if (one) {
 #pragma unroll
-                    for (unsigned j = 0; j < 4; ++j) ptx::mma_i8_ss_pair(d, dw + 2 * j, dx + 2 * j, idesc, i != 0 || j != 0 ? 1u : 0u);
-                    ptx::mma_commit_pair(empty_bar(stage), 3);
+                        for (unsigned j = 0; j < 4; ++j) ptx::mma_i8_ss_pair(d, dw + 2 * j, dx + 2 * j, idesc, i + j);
+                        ptx::mma_commit_pair(empty_bar(stage), 3);
+                    }
+                    __syncwarp();
                     if (++stage == stages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
-                if (ok) ptx::mma_commit_pair(acc_full_bar(acc), 3);
+                if (ok && one) ptx::mma_commit_pair(acc_full_bar(acc), 3);
+                __syncwarp();
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
             }
         }
-        __syncwarp();
     } else {
         const unsigned worker = warp - 2, quarter = warp % 4, turn = worker / 4;
         uint8_t* const boxes = smem + box_off + worker * 2 * kBoxBytes;
@@ -442,7 +485,7 @@ gemm_s8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     unsigned* const words = reinterpret_cast<unsigned*>(tail + kFewBarriers * 8);
     volatile unsigned* const abort_flag = words + 1;
 
-    const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const unsigned warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const unsigned rank = blockIdx.x % p.split, row0 = blockIdx.x / p.split * kRows;
     const int k0 = static_cast<int>(p.k_iters * rank / p.split), k1 = static_cast<int>(p.k_iters * (rank + 1) / p.split);
     const int iters = k1 - k0;
@@ -465,7 +508,7 @@ gemm_s8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     ptx::tc_fence_before_sync();
     __syncthreads();
     ptx::tc_fence_after_sync();
-    const uint32_t tmem = words[0];
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, words[0], 0);
     ptx::grid_launch_dependents();
 
     const auto load_w = [&](int i, int s) {
@@ -473,47 +516,55 @@ gemm_s8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         ptx::tma_load_2d(base + s * stage_bytes, &map_w, full_bar(s), (k0 + i) * static_cast<int>(kBK), static_cast<int>(row0));
     };
     const int early = p.early_w != 0 ? min(stages, iters) : 0;
-    if (warp == 0 && lane == 0) {
-        for (int i = 0; i < early; ++i) load_w(i, i);
+    if (warp == 0) {
+        const bool one = elect_one();
+        for (int i = 0; i < early; ++i) {
+            if (one) load_w(i, i);
+        }
+        __syncwarp();
     }
     ptx::grid_dependency_wait();
 
     if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
-            unsigned phase = 1;
-            for (int i = 0; i < iters; ++i) {
-                if (i >= stages && !wait_barrier(empty_bar(s), phase, abort_flag, p.status, kStatusProducerEmpty)) {
-                    grace_for_copies_in_flight();
-                    break;
-                }
+        const bool one = elect_one();
+        int s = 0;
+        unsigned phase = 1;
+        for (int i = 0; i < iters; ++i) {
+            if (i >= stages && !wait_warp(empty_bar(s), phase, abort_flag, p.status, kStatusProducerEmpty)) {
+                grace_for_copies_in_flight();
+                break;
+            }
+            if (one) {
                 if (i >= early) load_w(i, s);
                 ptx::tma_load_2d(base + s * stage_bytes + kWBytes, &map_x, full_bar(s), (k0 + i) * static_cast<int>(kBK), 0);
-                if (++s == stages) s = 0, phase ^= 1u;
             }
+            __syncwarp();
+            if (++s == stages) s = 0, phase ^= 1u;
         }
-        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = ptx::instr_desc_s8_s32acc(kRows, n_tok);
-            int s = 0;
-            unsigned phase = 0;
-            bool ok = true;
-            for (int i = 0; i < iters; ++i) {
-                if (!wait_barrier(full_bar(s), phase, abort_flag, p.status, kStatusMmaFull)) {
-                    ok = false;
-                    break;
-                }
-                ptx::tc_fence_after_sync();
-                const uint64_t dw = ptx::smem_desc_k_major_sw128(base + s * stage_bytes);
-                const uint64_t dx = ptx::smem_desc_k_major_sw128(base + s * stage_bytes + kWBytes);
-#pragma unroll
-                for (unsigned j = 0; j < 4; ++j) ptx::mma_i8_ss(tmem, dw + 2 * j, dx + 2 * j, idesc, i != 0 || j != 0 ? 1u : 0u);
-                if (i + stages < iters) ptx::mma_commit(empty_bar(s));
-                if (++s == stages) s = 0, phase ^= 1u;
+        const bool one = elect_one();
+        const uint32_t idesc = ptx::instr_desc_s8_s32acc(kRows, n_tok);
+        const uint64_t dw0 = ptx::smem_desc_k_major_sw128(base), dx0 = ptx::smem_desc_k_major_sw128(base + kWBytes);
+        const uint32_t step16 = stage_bytes >> 4;
+        int s = 0;
+        unsigned phase = 0;
+        bool ok = true;
+        for (int i = 0; i < iters; ++i) {
+            if (!wait_warp(full_bar(s), phase, abort_flag, p.status, kStatusMmaFull)) {
+                ok = false;
+                break;
             }
-            if (ok) ptx::mma_commit(acc_bar);
+            ptx::tc_fence_after_sync();
+            const uint64_t dw = dw0 + s * step16, dx = dx0 + s * step16;
+            if (one) {
+#pragma unroll
+                for (unsigned j = 0; j < 4; ++j) ptx::mma_i8_ss(tmem, dw + 2 * j, dx + 2 * j, idesc, i + j);
+                if (i + stages < iters) ptx::mma_commit(empty_bar(s));
+            }
+            __syncwarp();
+            if (++s == stages) s = 0, phase ^= 1u;
         }
+        if (ok && one) ptx::mma_commit(acc_bar);
         __syncwarp();
     } else {
         const unsigned quarter = warp % 4, turn = (warp - 2) / 4;

@@ -132,9 +132,22 @@ def _stream_ptr(stream) -> int:
     return int(torch.cuda.current_stream().cuda_stream) if raw is None else raw(torch.cuda.current_device())
 
 
+_TORCH = None
+
+
+def _torch():
+    """The torch module, imported at the first call that needs it (an import statement costs each call a lookup)."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+
+        _TORCH = torch
+    return _TORCH
+
+
 def _rows_of(t, device: int) -> bool:
-    """Whether t lies on cuda:`device` and its rows are contiguous."""
-    return t.device.type == "cuda" and t.device.index == device and (t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1)
+    """Whether t lies on cuda:`device` and its rows are contiguous. (get_device: a number, where t.device builds an object.)"""
+    return t.get_device() == device and (t.stride(-1) == 1 or t.shape[-1] == 1 or t.numel() == 0)
 
 
 def _ld(t, row: int) -> int:
@@ -143,9 +156,7 @@ def _ld(t, row: int) -> int:
 
 
 def _require_floats(t, n: int, device: int, who: str, what: str) -> None:
-    import torch
-
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device.type != "cuda" or t.device.index != device:
+    if t.dtype is not _torch().float32 or t.numel() != n or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{who}: {what} must be {n} contiguous float32 values on cuda:{device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
@@ -318,21 +329,17 @@ class Context:
         """The cudaStream_t of `stream`, or of the current stream of the context's device (which need not be the current one)."""
         if stream is not None:
             return int(stream.cuda_stream)
-        import torch
-
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        return int(torch.cuda.current_stream(self.device).cuda_stream) if raw is None else raw(self.device)
+        raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
+        return int(_torch().cuda.current_stream(self.device).cuda_stream) if raw is None else raw(self.device)
 
     def _rows_out(self, t: int, k: int, q, scales, who: str):
         """The int8 rows and their scales: new ones (rows of a multiple of 16 bytes, as gemm_s8 takes them), or the caller's after checks."""
-        import torch
-
         if q is None:
-            q = torch.empty((t, (k + 15) // 16 * 16), dtype=torch.int8, device=f"cuda:{self.device}")[:, :k]
-        elif q.shape != (t, k) or q.dtype != torch.int8 or not _rows_of(q, self.device):
+            q = _torch().empty((t, (k + 15) // 16 * 16), dtype=_torch().int8, device=f"cuda:{self.device}")[:, :k]
+        elif q.shape != (t, k) or q.dtype is not _torch().int8 or not _rows_of(q, self.device):
             raise ValueError(f"{who}: q must be int8 [{t}, {k}] on cuda:{self.device} with contiguous rows, not {q.dtype} {tuple(q.shape)}")
         if scales is None:
-            scales = torch.empty((t,), dtype=torch.float32, device=f"cuda:{self.device}")
+            scales = _torch().empty((t,), dtype=_torch().float32, device=f"cuda:{self.device}")
         else:
             _require_floats(scales, t, self.device, who, "scales")
         return q, scales
@@ -341,39 +348,34 @@ class Context:
         """The residual's addition (x += delta, in place; delta None: x is only read), the zero-centred RMSNorm and one int8 row with a
         float32 scale a token (sepal_b200_rms_norm_s8). x float32 [T, C], w float32 [C], delta float16 or float32 [T, C], col_scale float32
         [C] (smoothing factors); returns (q int8 [T, C], scales float32 [T])."""
-        import torch
-
-        if x.dim() != 2 or x.dtype != torch.float32 or not _rows_of(x, self.device):
-            raise ValueError(f"rms_norm_s8: x must be float32 [T, C] on cuda:{self.device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
+        torch, device = _torch(), self.device
+        if x.dim() != 2 or x.dtype is not torch.float32 or not _rows_of(x, device):
+            raise ValueError(f"rms_norm_s8: x must be float32 [T, C] on cuda:{device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
         t, c = x.shape
-        _require_floats(w, c, self.device, "rms_norm_s8", "w")
+        _require_floats(w, c, device, "rms_norm_s8", "w")
         if col_scale is not None:
-            _require_floats(col_scale, c, self.device, "rms_norm_s8", "col_scale")
-        half = 0
+            _require_floats(col_scale, c, device, "rms_norm_s8", "col_scale")
+        added, ld_added, half = None, 0, 0
         if delta is not None:
-            if delta.shape != x.shape or delta.dtype not in (torch.float16, torch.float32) or not _rows_of(delta, self.device):
-                raise ValueError(f"rms_norm_s8: delta must be float16 or float32 {tuple(x.shape)} on cuda:{self.device} with contiguous rows")
-            half = 1 if delta.dtype == torch.float16 else 0
-            if t > 1 and x.stride(0) < c:
-                raise ValueError("rms_norm_s8: the rows of x, which is updated in place, overlap")
+            if delta.shape != x.shape or delta.dtype not in (torch.float16, torch.float32) or not _rows_of(delta, device):
+                raise ValueError(f"rms_norm_s8: delta must be float16 or float32 {tuple(x.shape)} on cuda:{device} with contiguous rows")
+            added, ld_added, half = delta.data_ptr(), _ld(delta, c), 1 if delta.dtype is torch.float16 else 0
         q, scales = self._rows_out(t, c, q, scales, "rms_norm_s8")
-        _check(self._lib.sepal_b200_rms_norm_s8(self._h, x.data_ptr(), _ld(x, c), None if delta is None else delta.data_ptr(), 0 if delta is None else _ld(delta, c),
-                                                half, w.data_ptr(), None if col_scale is None else col_scale.data_ptr(), q.data_ptr(), _ld(q, c),
-                                                scales.data_ptr(), t, c, eps, self._stream(stream)))
+        _check(self._lib.sepal_b200_rms_norm_s8(self._h, x.data_ptr(), _ld(x, c), added, ld_added, half, w.data_ptr(), None if col_scale is None else col_scale.data_ptr(),
+                                                q.data_ptr(), _ld(q, c), scales.data_ptr(), t, c, eps, self._stream(stream)))
         return q, scales
 
     def quantize_tokens_s8(self, x, q=None, scales=None, *, col_scale=None, stream=None):
         """One int8 row with a float32 scale a token (sepal_b200_quantize_tokens_s8): x float16 or float32 [T, K] (times col_scale, float32
         [K]); returns (q int8 [T, K], scales float32 [T])."""
-        import torch
-
-        if x.dim() != 2 or x.dtype not in (torch.float16, torch.float32) or not _rows_of(x, self.device):
-            raise ValueError(f"quantize_tokens_s8: x must be float16 or float32 [T, K] on cuda:{self.device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
+        torch, device = _torch(), self.device
+        if x.dim() != 2 or x.dtype not in (torch.float16, torch.float32) or not _rows_of(x, device):
+            raise ValueError(f"quantize_tokens_s8: x must be float16 or float32 [T, K] on cuda:{device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
         t, k = x.shape
         if col_scale is not None:
-            _require_floats(col_scale, k, self.device, "quantize_tokens_s8", "col_scale")
+            _require_floats(col_scale, k, device, "quantize_tokens_s8", "col_scale")
         q, scales = self._rows_out(t, k, q, scales, "quantize_tokens_s8")
-        _check(self._lib.sepal_b200_quantize_tokens_s8(self._h, x.data_ptr(), _ld(x, k), 1 if x.dtype == torch.float16 else 0,
+        _check(self._lib.sepal_b200_quantize_tokens_s8(self._h, x.data_ptr(), _ld(x, k), 1 if x.dtype is torch.float16 else 0,
                                                        None if col_scale is None else col_scale.data_ptr(), q.data_ptr(), _ld(q, k), scales.data_ptr(),
                                                        t, k, self._stream(stream)))
         return q, scales
@@ -381,25 +383,27 @@ class Context:
     def gemm_s8(self, xq, sx, wq, sw, y=None, *, epilogue: int = STORE, y_half: bool = True, config: int = -1, stream=None):
         """y = epilogue(float(xq @ wq.T) * sx[:, None] * sw): xq int8 [T, K] with sx float32 [T] (rms_norm_s8, quantize_tokens_s8), wq int8
         [N, K] with sw float32 [N] (quantize_rows_s8). The sums are exact integers (sepal_b200_gemm_s8)."""
-        import torch
-
-        if xq.dim() != 2 or wq.dim() != 2 or xq.dtype != torch.int8 or wq.dtype != torch.int8 or not _rows_of(xq, self.device) or not _rows_of(wq, self.device):
-            raise ValueError(f"gemm_s8: xq and wq must be int8 matrices on cuda:{self.device} with contiguous rows")
+        torch, device = _torch(), self.device
+        if xq.dim() != 2 or wq.dim() != 2 or xq.dtype is not torch.int8 or wq.dtype is not torch.int8 or not _rows_of(xq, device) or not _rows_of(wq, device):
+            raise ValueError(f"gemm_s8: xq and wq must be int8 matrices on cuda:{device} with contiguous rows")
         t, k = xq.shape
-        n = wq.shape[0]
-        if wq.shape[1] != k:
+        n, wk = wq.shape
+        if wk != k:
             raise ValueError(f"gemm_s8: xq is [{t}, {k}] but wq is {tuple(wq.shape)}: the inner dimensions must agree")
-        _require_floats(sx, t, self.device, "gemm_s8", "sx")
-        _require_floats(sw, n, self.device, "gemm_s8", "sw")
-        if y is not None:
-            y_half = y.dtype == torch.float16
-        elif epilogue == ADD:
-            raise ValueError("gemm_s8: epilogue ADD updates an output that the caller gives")
+        _require_floats(sx, t, device, "gemm_s8", "sx")
+        _require_floats(sw, n, device, "gemm_s8", "sw")
         columns = n // 2 if epilogue == SWIGLU else n
-        y = self._out(xq, columns, y, y_half)
-        # (a lone row's stride is never used: any that the kernels take)
-        _check(self._lib.sepal_b200_gemm_s8(self._h, xq.data_ptr(), _ld(xq, (k + 15) // 16 * 16), sx.data_ptr(), wq.data_ptr(), _ld(wq, (k + 15) // 16 * 16),
-                                            sw.data_ptr(), y.data_ptr(), _ld(y, columns), 1 if y_half else 0, t, n, k, epilogue, config, self._stream(stream)))
+        if y is None:
+            if epilogue == ADD:
+                raise ValueError("gemm_s8: epilogue ADD updates an output that the caller gives")
+            y = torch.empty((t, columns), dtype=torch.float16 if y_half else torch.float32, device=xq.device)
+        else:
+            y_half = y.dtype is torch.float16
+            if y.shape != (t, columns) or not (y_half or y.dtype is torch.float32) or not _rows_of(y, device):
+                raise ValueError(f"gemm_s8: the output must be float16 or float32 [{t}, {columns}] on cuda:{device} with contiguous rows, not {y.dtype} {tuple(y.shape)}")
+        row = (k + 15) // 16 * 16  # (a lone row's stride is never used: one that the kernels take)
+        _check(self._lib.sepal_b200_gemm_s8(self._h, xq.data_ptr(), _ld(xq, row), sx.data_ptr(), wq.data_ptr(), _ld(wq, row), sw.data_ptr(), y.data_ptr(),
+                                            _ld(y, columns), 1 if y_half else 0, t, n, k, epilogue, config, self._stream(stream)))
         return y
 
     def pack_gate_up(self, stacked, stream=None):

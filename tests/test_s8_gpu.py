@@ -448,7 +448,7 @@ def test_refusals_of_the_library(ctx):
                                       ld_y, 0, t, n, k, epilogue, config, None)
 
     for call in (lambda: norm(ld_x=63), lambda: norm(ld_q=63), lambda: norm(delta=x.data_ptr(), ld_delta=63), lambda: norm(w=None), lambda: norm(cols=0),
-                 lambda: norm(eps=0.0), lambda: norm(eps=-1.0), lambda: norm(eps=float("nan")), lambda: norm(eps=float("inf")), lambda: norm(rows=1 << 31),
+                 lambda: norm(ld_x=0), lambda: norm(eps=0.0), lambda: norm(eps=-1.0), lambda: norm(eps=float("nan")), lambda: norm(eps=float("inf")), lambda: norm(rows=1 << 31),
                  lambda: multiply(ld_x=72), lambda: multiply(ld_x=48), lambda: multiply(ld_w=72), lambda: multiply(ld_y=63), lambda: multiply(k=0),
                  lambda: multiply(n=0), lambda: multiply(k=1 << 17, ld_x=1 << 17, ld_w=1 << 17), lambda: multiply(epilogue=2), lambda: multiply(epilogue=3),
                  lambda: multiply(xq=q.data_ptr() + 8), lambda: multiply(sx=None), lambda: multiply(config=0), lambda: multiply(config=-2), lambda: multiply(config=512),

@@ -50,8 +50,6 @@ def test_shapes_types_and_strides_are_refused(bare, monkeypatch):
     for bad in (torch.zeros(4, 63), torch.zeros(3, 64), torch.zeros(4, 64).bfloat16()):
         with pytest.raises(ValueError, match="delta must be"):
             bare.rms_norm_s8(x, w, delta=bad)
-    with pytest.raises(ValueError, match="overlap"):
-        bare.rms_norm_s8(torch.zeros(64).expand(4, 64), w, delta=x)
     for bad in (torch.zeros(4, 64), torch.zeros(4, 48, dtype=torch.int8), torch.zeros(64, 4, dtype=torch.int8).t()):
         with pytest.raises(ValueError, match="q must be"):
             bare.rms_norm_s8(x, w, bad, torch.zeros(4))
@@ -72,7 +70,7 @@ def test_shapes_types_and_strides_are_refused(bare, monkeypatch):
         bare.gemm_s8(xq, sx, wq, sw, epilogue=sb.ADD)
     with pytest.raises(ValueError, match="output must be"):
         bare.gemm_s8(xq, sx, wq, sw, torch.zeros(4, 9))
-    with pytest.raises(ValueError, match="float16 or float32"):
+    with pytest.raises(ValueError, match="output must be float16 or float32"):
         bare.gemm_s8(xq, sx, wq, sw, torch.zeros(4, 8).bfloat16())
 
 
