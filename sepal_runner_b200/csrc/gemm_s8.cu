@@ -693,17 +693,40 @@ void launch_few(const Context& ctx, const std::int8_t* x, std::size_t ld_x, cons
     count_launch();
 }
 
-// Tokens to a tile of the pair kernel.
-unsigned pick_tokens(unsigned pairs, std::size_t t, std::size_t n, std::size_t k_iters) {
-    const std::size_t n_tiles = (n + 255) / 256;
-    unsigned best = 256;
-    double best_cost = 0.0;
-    for (unsigned bt = 32; bt <= 256; bt += 32) {
-        const std::size_t tiles = (t + bt - 1) / bt * n_tiles, waves = (tiles + pairs - 1) / pairs;
-        const double cost = static_cast<double>(waves) * (static_cast<double>(k_iters) * (256.0 + bt) + 1000.0);
-        if (best_cost == 0.0 || cost <= best_cost) best = bt, best_cost = cost;
+// The automatic choice: the kernel, and the pair kernel's tokens to a tile, by an estimate in microseconds fitted to every width and every split
+// of k over thirteen projections (1024 to 24576 weight rows, k from 1024 to 12288) at 21 token counts from 1 to 4096 on 148 SMs: what it
+// picks is on average 2 % slower than the best of them, on single shapes of a few microseconds up to 33 %.
+//   - A step of the pair kernel is 2 bt clocks of tensor cores, or 180 + 0.6 bt where the boxes' arrival bounds it (tiles under 128 tokens); a
+//     wave of tiles has about 600 clocks of its own (first boxes, the last tile's epilogue).
+//   - Cutting k over a cluster costs 0.028 us a token in the exchange of the sums: it wins where a few weight rows have a long k (2560 x 9728, one
+//     token: 12.3 us on ten pairs, 7.4 cut in eight; level at about 200 tokens; 24576 x 4096: 18.5 on pairs from one token on).
+//   - Neither reads the weights faster than the memory does, about 6.5 TB/s.
+struct Choice {
+    bool few = false;
+    unsigned bt = 32;
+    FewSchedule parts;
+};
+Choice choose(unsigned sm_count, std::size_t t, std::size_t n, std::size_t k) {
+    const std::size_t iters = (k + kBK - 1) / kBK, pairs = sm_count / 2;
+    const double reading = static_cast<double>(n) * static_cast<double>(k) / 6.5e6;
+    Choice c;
+    double best = 0.0;
+    for (unsigned bt = 32; bt <= 256 && bt < t + 32; bt += 32) {
+        const std::size_t tiles = (t + bt - 1) / bt * ((n + 255) / 256), waves = (tiles + pairs - 1) / pairs;
+        const double step = 2.0 * bt > 180.0 + 0.6 * bt ? 2.0 * bt : 180.0 + 0.6 * bt;
+        const double us = static_cast<double>(waves) * (static_cast<double>(iters) * step + 600.0) / 1900.0;
+        if (best == 0.0 || us <= best) best = us, c.bt = bt;
     }
-    return best;
+    if (t > kFewMaxRows) return c;
+    // up to 32 tokens two CTAs to an SM, above one, whose ring is deeper (2560 x 9728, 64 tokens: 10.9 and 9.8 us)
+    const FewSchedule parts = few_schedule(sm_count, t <= 32 ? t : 129, n, k, true);
+    const std::size_t ctas = (n + kRows - 1) / kRows * parts.split, room = static_cast<std::size_t>(sm_count) * parts.slots;
+    const double cut = 0.11 * static_cast<double>((ctas + room - 1) / room) * static_cast<double>((iters + parts.split - 1) / parts.split);
+    if (3.2 + (cut > reading ? cut : reading) + 0.028 * static_cast<double>(t) < 3.6 + (best > reading ? best : reading)) {
+        c.few = true;
+        c.parts = parts;
+    }
+    return c;
 }
 
 }  // namespace
@@ -716,9 +739,9 @@ void launch_gemm_s8(Context& ctx, const std::int8_t* x, std::size_t ld_x, const 
                                     std::to_string(k) + "] (K from 1 to 131071, the strides of X and W multiples of 16 that hold a row, that of Y one that "
                                     "holds a row, SwiGLU needs N a multiple of 128)");
     if (t > 0x7FFFFFFFu || n > 0x7FFFFFFFu) throw std::invalid_argument("launch_gemm_s8: dimension beyond 2^31");
-    const bool few = config >= kFewConfig, forced_pair = config >= 512 && !few;
-    const int parts = few ? (config - kFewConfig) % 16 : 0, slots = few && config - kFewConfig >= 16 ? 1 : 2;
-    if (config < -1 || (config >= 0 && config < 512) || (forced_pair && (config - 512 < 32 || config - 512 > 256 || (config - 512) % 32 != 0)) ||
+    const bool few = config >= kFewConfig, pair = config >= 512 && !few;
+    const int parts = few ? (config - kFewConfig) % 16 : 1, slots = few && config - kFewConfig >= 16 ? 1 : 2;
+    if (config < -1 || (config >= 0 && config < 512) || (pair && (config - 512 < 32 || config - 512 > 256 || (config - 512) % 32 != 0)) ||
         (few && (config - kFewConfig >= 32 || parts < 1 || parts > 8)))
         throw std::invalid_argument("launch_gemm_s8: config is -1, 512 + w (w tokens to a tile: a multiple of 32 up to 256) or 1024 + s, 1024 + 16 + s (s parts "
                                     "of k, 1 to 8)");
@@ -744,19 +767,19 @@ void launch_gemm_s8(Context& ctx, const std::int8_t* x, std::size_t ld_x, const 
     p.y_half = y_half ? 1u : 0u;
     p.vec_ok = reinterpret_cast<std::uintptr_t>(y) % 16 == 0 && ld_y * (y_half ? 2 : 4) % 16 == 0 ? 1u : 0u;
     p.early_w = ctx.static_weights ? 1u : 0u;
-    if (few || (config == -1 && t <= 128)) {
-        FewSchedule sched;
-        if (few) {
-            sched.split = static_cast<unsigned>(parts);
-            sched.slots = static_cast<unsigned>(slots);
-        } else {
-            sched = few_schedule(static_cast<unsigned>(ctx.sm_count), t, n, k, true);
-        }
-        launch_few(ctx, x, ld_x, w, ld_w, p, k, sched, stream);
-        return;
+    Choice c;
+    if (config == -1) {
+        c = choose(static_cast<unsigned>(ctx.sm_count), t, n, k);
+    } else {
+        c.few = few;
+        c.bt = static_cast<unsigned>(config - 512);
+        c.parts.split = static_cast<unsigned>(parts);
+        c.parts.slots = static_cast<unsigned>(slots);
     }
-    launch_pair(ctx, x, ld_x, w, ld_w, p, k,
-                forced_pair ? static_cast<unsigned>(config - 512) : pick_tokens(static_cast<unsigned>(ctx.sm_count) / 2, t, n, p.k_iters), stream);
+    if (c.few)
+        launch_few(ctx, x, ld_x, w, ld_w, p, k, c.parts, stream);
+    else
+        launch_pair(ctx, x, ld_x, w, ld_w, p, k, c.bt, stream);
 }
 
 }  // namespace sepal::b200

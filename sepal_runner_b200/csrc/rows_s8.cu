@@ -4,11 +4,15 @@
 // v / max |v| = u / max |u|: the bytes do not depend on r at all, only the row's scale does. So the sum of squares and the maximum are taken
 // in ONE pass over the registers and the block meets at one barrier, where norm, then maximum, then rounding would meet at two.
 //
-// What bounds it: memory (4 to 13 bytes a value, under ten instructions). A block owns a row and keeps it in registers between the
-// reduction and the rounding: every thread has its up to four 16-byte loads in flight at once (a 2560-wide float32 row is 160 threads,
-// a 9728-wide binary16 row 320), and five to ten blocks to an SM hide one another's barrier. Rows wider than 1024 threads hold are read
-// again behind the barrier (from the L2). Rows that are not aligned to the vectors, or whose length is odd, take a kernel of
-// single-value accesses.
+// What bounds it: memory (3 to 13 bytes a value, under ten instructions). A block owns a row and keeps it in registers between the
+// reduction and the rounding, a thread up to four vectors of 16 bytes (a 2560-wide float32 row is 160 threads, a 9728-wide binary16 row
+// 320), all of whose loads are issued before the first is used and leave the L1 to the gains. With two vectors to a thread a single row
+// is 0.3 us faster and 4096 rows of 4096 values 3.6 us slower (23.1 and 19.5); a ring of rows in shared memory, filled by bulk copies
+// while groups of warps round, was built and was 10 to 30 % slower but for 48 KB rows without gains. Rows wider than 768 threads hold are
+// read again behind the barrier (from the L2). Rows that are not aligned to the vectors, or whose length is odd, take a kernel of single-value
+// accesses. Measured alone, back to back, against the memory's 6.56 TB/s: 4096 x 2560, float32 delta 24.1 us (86 %), binary16 delta 20.5 (86 %);
+// 4096 x 4096 without 19.5 (66 %); quantise 4096 x 9728 binary16 22.9 (80 %), 4096 x 12288 float32 46.1 (83 %); 900 x 2560, binary16 delta 7.0
+// (55 %: half of it a launch's start and end); one row 2.1 to 2.6 us.
 #include "rows_s8.hpp"
 
 #include <cmath>
@@ -29,7 +33,7 @@ void count_launch();
 namespace {
 
 constexpr int kHeld = 4;                 // vectors a thread keeps
-constexpr unsigned kMaxThreads = 1024;
+constexpr unsigned kMaxThreads = 768, kNarrowThreads = 512;
 constexpr unsigned kInfBits = 0x7F800000u;
 
 struct RowsParams {
@@ -46,6 +50,9 @@ struct RowsParams {
     float eps;
 };
 
+// Both forms give a row to the same number of threads, thread i the vectors i, i + threads, ..., and adds the threads' sums in the same order:
+// a row's scale has the same bits whichever form its call took.
+//
 // What the block's threads make of a row: the sum of x^2 and the largest |u| as the bit pattern of a non-negative float, which orders like
 // an unsigned integer, infinities and NaN last. One barrier.
 template <bool NORM>
@@ -109,11 +116,32 @@ __device__ __forceinline__ void widen(const uint4& raw, float (&v)[8]) {
         v[2 * i] = f.x, v[2 * i + 1] = f.y;
     }
 }
+__device__ __forceinline__ float4 product(const float4& a, const float4& b) {
+    return make_float4(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y), __fmul_rn(a.z, b.z), __fmul_rn(a.w, b.w));
+}
+__device__ __forceinline__ float square_into(float sum, const float4& v) {
+    return __fmaf_rn(v.w, v.w, __fmaf_rn(v.z, v.z, __fmaf_rn(v.y, v.y, __fmaf_rn(v.x, v.x, sum))));
+}
+// 16 bytes that are read once: they leave the L1 to the gains, which every row reads again.
+__device__ __forceinline__ uint4 load_once(const void* at) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load_once_f32(const void* at) {
+    const uint4 v = load_once(at);
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// DELTA: 0 none, 1 binary16, 2 float32. A vector is four values.
-template <int DELTA>
-__global__ void __launch_bounds__(kMaxThreads) rms_norm_s8_kernel(const RowsParams p) {
+__device__ __forceinline__ unsigned largest_of(unsigned top, const float4& u) {
+    return max(max(top, max(magnitude(u.x), magnitude(u.y))), max(magnitude(u.z), magnitude(u.w)));
+}
+
+// DELTA: 0 none, 1 binary16, 2 float32. A vector is four values. WIDE: blocks of more than kNarrowThreads, held to registers that let two
+// of them onto an SM (12288 float32 values a row, 4096 rows: 63 us with one, 46 with two); narrow blocks are faster with all they ask for.
+template <int DELTA, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? kMaxThreads : kNarrowThreads, WIDE ? 2 : 1) rms_norm_s8_kernel(const RowsParams p) {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const std::size_t row = blockIdx.x;
@@ -122,7 +150,7 @@ __global__ void __launch_bounds__(kMaxThreads) rms_norm_s8_kernel(const RowsPara
     const float4* const gain = reinterpret_cast<const float4*>(p.w);
     const float4* const smooth = reinterpret_cast<const float4*>(p.col_scale);
     const auto added = [&](unsigned c) {
-        float4 v = xr[c];
+        float4 v = load_once_f32(xr + c);
         if constexpr (DELTA != 0) {
             float4 d;
             if constexpr (DELTA == 1) {
@@ -130,24 +158,18 @@ __global__ void __launch_bounds__(kMaxThreads) rms_norm_s8_kernel(const RowsPara
                 const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
                 d = make_float4(lo.x, lo.y, hi.x, hi.y);
             } else {
-                d = reinterpret_cast<const float4*>(static_cast<const float*>(p.delta) + row * p.ld_delta)[c];
+                d = load_once_f32(reinterpret_cast<const float4*>(static_cast<const float*>(p.delta) + row * p.ld_delta) + c);
             }
             v = make_float4(__fadd_rn(v.x, d.x), __fadd_rn(v.y, d.y), __fadd_rn(v.z, d.z), __fadd_rn(v.w, d.w));
         }
         return v;
     };
     const auto gained = [&](const float4& v, unsigned c) {
-        const float4 g = gain[c];
-        float4 u = make_float4(__fmul_rn(v.x, __fadd_rn(1.0f, g.x)), __fmul_rn(v.y, __fadd_rn(1.0f, g.y)), __fmul_rn(v.z, __fadd_rn(1.0f, g.z)),
-                               __fmul_rn(v.w, __fadd_rn(1.0f, g.w)));
-        if (smooth != nullptr) {
-            const float4 m = smooth[c];
-            u = make_float4(__fmul_rn(u.x, m.x), __fmul_rn(u.y, m.y), __fmul_rn(u.z, m.z), __fmul_rn(u.w, m.w));
-        }
-        return u;
+        float4 g = gain[c];
+        g = make_float4(__fadd_rn(1.0f, g.x), __fadd_rn(1.0f, g.y), __fadd_rn(1.0f, g.z), __fadd_rn(1.0f, g.w));
+        if (smooth != nullptr) g = product(g, smooth[c]);
+        return product(v, g);
     };
-    const auto square = [](float sum, const float4& v) { return __fmaf_rn(v.w, v.w, __fmaf_rn(v.z, v.z, __fmaf_rn(v.y, v.y, __fmaf_rn(v.x, v.x, sum)))); };
-    const auto largest = [](unsigned top, const float4& u) { return max(max(top, max(magnitude(u.x), magnitude(u.y))), max(magnitude(u.z), magnitude(u.w))); };
 
     float4 held[kHeld];
 #pragma unroll
@@ -162,16 +184,16 @@ __global__ void __launch_bounds__(kMaxThreads) rms_norm_s8_kernel(const RowsPara
         const unsigned c = threadIdx.x + blockDim.x * i;
         if (c < vecs) {
             if constexpr (DELTA != 0) xr[c] = held[i];
-            sum = square(sum, held[i]);
+            sum = square_into(sum, held[i]);
             held[i] = gained(held[i], c);
-            top = largest(top, held[i]);
+            top = largest_of(top, held[i]);
         }
     }
     for (unsigned c = threadIdx.x + blockDim.x * kHeld; c < vecs; c += blockDim.x) {
         const float4 v = added(c);
         if constexpr (DELTA != 0) xr[c] = v;
-        sum = square(sum, v);
-        top = largest(top, gained(v, c));
+        sum = square_into(sum, v);
+        top = largest_of(top, gained(v, c));
     }
     reduce_row<true>(sum, top);
     const RowScale s = row_scale<true>(sum, top, p);
@@ -188,9 +210,34 @@ __global__ void __launch_bounds__(kMaxThreads) rms_norm_s8_kernel(const RowsPara
     if (threadIdx.x == 0) p.scales[row] = s.scale;
 }
 
-// Quantisation alone. A vector is 16 bytes of x: eight binary16 values or four float32 ones, kept as they came.
+// A vector of a row to quantise is 16 bytes of x, eight binary16 values or four float32 ones: its values, scaled.
 template <bool HALF>
-__global__ void __launch_bounds__(kMaxThreads) quantize_tokens_s8_kernel(const RowsParams p) {
+__device__ __forceinline__ void row_values(const uint4& raw, const float4* smooth, unsigned c, float (&v)[HALF ? 8 : 4]) {
+    if constexpr (HALF) {
+        widen(raw, v);
+    } else {
+        v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y), v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+    }
+    if (smooth == nullptr) return;
+#pragma unroll
+    for (int h = 0; h < (HALF ? 2 : 1); ++h) {
+        const float4 m = smooth[c * (HALF ? 2 : 1) + h];
+        v[4 * h] = __fmul_rn(v[4 * h], m.x), v[4 * h + 1] = __fmul_rn(v[4 * h + 1], m.y);
+        v[4 * h + 2] = __fmul_rn(v[4 * h + 2], m.z), v[4 * h + 3] = __fmul_rn(v[4 * h + 3], m.w);
+    }
+}
+template <bool HALF>
+__device__ __forceinline__ void store_bytes(std::int8_t* q, unsigned c, const float (&v)[HALF ? 8 : 4], const RowScale& s) {
+    const unsigned lo = four_bytes(v[0], v[1], v[2], v[3], s);
+    if constexpr (HALF)
+        reinterpret_cast<uint2*>(q)[c] = make_uint2(lo, four_bytes(v[4], v[5], v[6], v[7], s));
+    else
+        reinterpret_cast<unsigned*>(q)[c] = lo;
+}
+
+// Quantisation alone, a block to a row; the vectors are kept as they came.
+template <bool HALF, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? kMaxThreads : kNarrowThreads, WIDE ? 2 : 1) quantize_tokens_s8_kernel(const RowsParams p) {
     constexpr int kValues = HALF ? 8 : 4;
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
@@ -198,24 +245,9 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_tokens_s8_kernel(const R
     const unsigned vecs = static_cast<unsigned>(p.cols / kValues);
     const uint4* const xr = reinterpret_cast<const uint4*>(static_cast<const char*>(p.x) + row * p.ld_x * (HALF ? 2 : 4));
     const float4* const smooth = reinterpret_cast<const float4*>(p.col_scale);
-    const auto values = [&](const uint4& raw, unsigned c, float (&v)[kValues]) {
-        if constexpr (HALF) {
-            widen(raw, v);
-        } else {
-            v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y), v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
-        }
-        if (smooth != nullptr) {
-#pragma unroll
-            for (int j = 0; j < kValues / 4; ++j) {
-                const float4 m = smooth[c * (kValues / 4) + j];
-                v[4 * j] = __fmul_rn(v[4 * j], m.x), v[4 * j + 1] = __fmul_rn(v[4 * j + 1], m.y);
-                v[4 * j + 2] = __fmul_rn(v[4 * j + 2], m.z), v[4 * j + 3] = __fmul_rn(v[4 * j + 3], m.w);
-            }
-        }
-    };
     const auto largest = [&](unsigned top, const uint4& raw, unsigned c) {
         float v[kValues];
-        values(raw, c, v);
+        row_values<HALF>(raw, smooth, c, v);
 #pragma unroll
         for (int j = 0; j < kValues; ++j) top = max(top, magnitude(v[j]));
         return top;
@@ -224,7 +256,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_tokens_s8_kernel(const R
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const unsigned c = threadIdx.x + blockDim.x * i;
-        held[i] = c < vecs ? xr[c] : make_uint4(0u, 0u, 0u, 0u);
+        if (c < vecs) held[i] = load_once(xr + c);
     }
     unsigned top = 0;
 #pragma unroll
@@ -238,12 +270,8 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_tokens_s8_kernel(const R
     const RowScale s = row_scale<false>(0.0f, top, p);
     const auto store = [&](const uint4& raw, unsigned c) {
         float v[kValues];
-        values(raw, c, v);
-        const unsigned lo = four_bytes(v[0], v[1], v[2], v[3], s);
-        if constexpr (HALF)
-            reinterpret_cast<uint2*>(p.q + row * p.ld_q)[c] = make_uint2(lo, four_bytes(v[4], v[5], v[6], v[7], s));
-        else
-            reinterpret_cast<unsigned*>(p.q + row * p.ld_q)[c] = lo;
+        row_values<HALF>(raw, smooth, c, v);
+        store_bytes<HALF>(p.q + row * p.ld_q, c, v, s);
     };
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
@@ -254,9 +282,9 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_tokens_s8_kernel(const R
     if (threadIdx.x == 0) p.scales[row] = s.scale;
 }
 
-// Any alignment and any length, a value at a time; the same arithmetic. A thread reads back only what it wrote itself.
+// Any alignment and any length, a value at a time; the same arithmetic in the same order. A thread reads back only what it wrote itself.
 template <bool NORM, bool HALF, int DELTA>
-__global__ void __launch_bounds__(256) rows_s8_any_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kMaxThreads) rows_s8_any_kernel(const RowsParams p) {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const std::size_t row = blockIdx.x;
@@ -267,25 +295,34 @@ __global__ void __launch_bounds__(256) rows_s8_any_kernel(const RowsParams p) {
             return static_cast<const float*>(p.x)[row * p.ld_x + c];
     };
     const auto gained = [&](float v, std::size_t c) {
-        if constexpr (NORM) v = __fmul_rn(v, __fadd_rn(1.0f, p.w[c]));
+        if constexpr (NORM) {
+            const float g = __fadd_rn(1.0f, p.w[c]);
+            return __fmul_rn(v, p.col_scale != nullptr ? __fmul_rn(g, p.col_scale[c]) : g);
+        }
         return p.col_scale != nullptr ? __fmul_rn(v, p.col_scale[c]) : v;
     };
     float sum = 0.0f;
     unsigned top = 0;
-    for (std::size_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
-        float v = fetch(c);
-        if constexpr (DELTA != 0) {
-            const std::size_t at = row * p.ld_delta + c;
-            v = __fadd_rn(v, DELTA == 1 ? __half2float(static_cast<const __half*>(p.delta)[at]) : static_cast<const float*>(p.delta)[at]);
-            const_cast<float*>(static_cast<const float*>(p.x))[row * p.ld_x + c] = v;
+    for (std::size_t first = 4 * static_cast<std::size_t>(threadIdx.x); first < p.cols; first += 4 * static_cast<std::size_t>(blockDim.x)) {
+        const std::size_t end = first + 4 < p.cols ? first + 4 : p.cols;
+        for (std::size_t c = first; c < end; ++c) {
+            float v = fetch(c);
+            if constexpr (DELTA != 0) {
+                const std::size_t at = row * p.ld_delta + c;
+                v = __fadd_rn(v, DELTA == 1 ? __half2float(static_cast<const __half*>(p.delta)[at]) : static_cast<const float*>(p.delta)[at]);
+                const_cast<float*>(static_cast<const float*>(p.x))[row * p.ld_x + c] = v;
+            }
+            if constexpr (NORM) sum = __fmaf_rn(v, v, sum);
+            top = max(top, magnitude(gained(v, c)));
         }
-        if constexpr (NORM) sum = __fmaf_rn(v, v, sum);
-        top = max(top, magnitude(gained(v, c)));
     }
     reduce_row<NORM>(sum, top);
     const RowScale s = row_scale<NORM>(sum, top, p);
-    for (std::size_t c = threadIdx.x; c < p.cols; c += blockDim.x)
-        p.q[row * p.ld_q + c] = s.finite ? static_cast<std::int8_t>(rounded(gained(fetch(c), c), s) & 0xFFu) : std::int8_t{0};
+    for (std::size_t first = 4 * static_cast<std::size_t>(threadIdx.x); first < p.cols; first += 4 * static_cast<std::size_t>(blockDim.x)) {
+        const std::size_t end = first + 4 < p.cols ? first + 4 : p.cols;
+        for (std::size_t c = first; c < end; ++c)
+            p.q[row * p.ld_q + c] = s.finite ? static_cast<std::int8_t>(rounded(gained(fetch(c), c), s) & 0xFFu) : std::int8_t{0};
+    }
     if (threadIdx.x == 0) p.scales[row] = s.scale;
 }
 
@@ -318,11 +355,13 @@ void launch_rms_norm_s8(const Context& ctx, float* x, std::size_t ld_x, const vo
                          (col_scale == nullptr || aligned(col_scale, 16)) && (kind == 0 || (ld_delta % 4 == 0 && aligned(delta, delta_half ? 8 : 16)));
     const dim3 grid(static_cast<unsigned>(rows));
     if (vectors) {
-        const auto kernel = kind == 0 ? rms_norm_s8_kernel<0> : kind == 1 ? rms_norm_s8_kernel<1> : rms_norm_s8_kernel<2>;
-        launch_kernel(kernel, grid, dim3(threads_for(cols / 4)), 0, stream, "rms_norm_s8_kernel launch", p);
+        const unsigned threads = threads_for(cols / 4);
+        const auto narrow = kind == 0 ? rms_norm_s8_kernel<0, false> : kind == 1 ? rms_norm_s8_kernel<1, false> : rms_norm_s8_kernel<2, false>;
+        const auto wide = kind == 0 ? rms_norm_s8_kernel<0, true> : kind == 1 ? rms_norm_s8_kernel<1, true> : rms_norm_s8_kernel<2, true>;
+        launch_kernel(threads > kNarrowThreads ? wide : narrow, grid, dim3(threads), 0, stream, "rms_norm_s8_kernel launch", p);
     } else {
         const auto kernel = kind == 0 ? rows_s8_any_kernel<true, false, 0> : kind == 1 ? rows_s8_any_kernel<true, false, 1> : rows_s8_any_kernel<true, false, 2>;
-        launch_kernel(kernel, grid, dim3(256), 0, stream, "rows_s8_any_kernel launch", p);
+        launch_kernel(kernel, grid, dim3(threads_for((cols + 3) / 4)), 0, stream, "rows_s8_any_kernel launch", p);
     }
     count_launch();
 }
@@ -338,11 +377,15 @@ void launch_quantize_tokens_s8(const Context& ctx, const void* x, std::size_t ld
     const bool vectors = cols % values == 0 && ld_x % values == 0 && ld_q % values == 0 && aligned(x, 16) && aligned(q, values) &&
                          (col_scale == nullptr || aligned(col_scale, 16));
     const dim3 grid(static_cast<unsigned>(rows));
-    if (vectors)
-        launch_kernel(x_half ? quantize_tokens_s8_kernel<true> : quantize_tokens_s8_kernel<false>, grid, dim3(threads_for(cols / values)), 0, stream,
-                      "quantize_tokens_s8_kernel launch", p);
-    else
-        launch_kernel(x_half ? rows_s8_any_kernel<false, true, 0> : rows_s8_any_kernel<false, false, 0>, grid, dim3(256), 0, stream, "rows_s8_any_kernel launch", p);
+    if (vectors) {
+        const unsigned threads = threads_for(cols / values);
+        const auto narrow = x_half ? quantize_tokens_s8_kernel<true, false> : quantize_tokens_s8_kernel<false, false>;
+        const auto wide = x_half ? quantize_tokens_s8_kernel<true, true> : quantize_tokens_s8_kernel<false, true>;
+        launch_kernel(threads > kNarrowThreads ? wide : narrow, grid, dim3(threads), 0, stream, "quantize_tokens_s8_kernel launch", p);
+    } else {
+        const auto kernel = x_half ? rows_s8_any_kernel<false, true, 0> : rows_s8_any_kernel<false, false, 0>;
+        launch_kernel(kernel, grid, dim3(threads_for((cols + 3) / 4)), 0, stream, "rows_s8_any_kernel launch", p);
+    }
     count_launch();
 }
 

@@ -3,7 +3,7 @@ formulas in 64 bits.
 
 Tolerances. A byte is the rounding of u * 127 / max|u|: u carries at most three float32 roundings (1 + w, the two products), 127 / max one, their
 product one, max one of u's three: under 8 halves of a float32 step, so the byte is within 0.5 + 127 * 8 * 2^-24 of the exact quotient. A scale adds the
-sum of squares (under 40 additions in any chain, halved by the square root) and four roundings: 32 * 2^-24 relative. The multiply's sums are
+sum of squares (under 60 additions in any chain, halved by the square root) and four roundings: 40 * 2^-24 relative. The multiply's sums are
 exact integers, and its two products by the scales can be repeated in float32 to the bit."""
 import ctypes as C
 
@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 
 STEP = 2.0**-24
 BYTE = 0.5 + 127 * 8 * STEP
-SCALE = 32 * STEP
+SCALE = 40 * STEP
 
 
 def generator(seed):
@@ -50,8 +50,8 @@ def guarded_rows(t, c, pad=16, offset=0):
     return q, untouched
 
 
-# widths: a lone vector, not whole warps, the served models' (1024 .. 4096), what 1024 threads hold to the value and one vector more, odd ones
-WIDTHS = [4, 132, 1024, 2560, 4096, 16384, 16388, 20000, 1, 7, 1023, 2563]
+# widths: a lone vector, not whole warps, the served models' (1024 .. 4096), what 512 and 768 threads hold to the vector and one more, odd ones
+WIDTHS = [4, 132, 1024, 2560, 4096, 8192, 8196, 12288, 12292, 20000, 1, 7, 1023, 2563, 12289]
 
 
 @pytest.mark.parametrize("cols", WIDTHS)
@@ -77,7 +77,7 @@ def test_norm(ctx, cols, delta):
         assert scales[0] == 7 and scales[t + 1] == 7
 
 
-@pytest.mark.parametrize("cols", [8, 264, 3584, 9728, 12288, 32768, 32776, 40000, 1, 7, 1023, 2564])
+@pytest.mark.parametrize("cols", [8, 264, 3584, 9728, 12288, 16384, 16392, 24576, 24584, 40000, 1, 7, 1023, 2564, 24577])
 @pytest.mark.parametrize("half", [True, False])
 def test_quantiser(ctx, cols, half):
     gen = generator(cols + 1)
@@ -98,8 +98,7 @@ def test_quantiser(ctx, cols, half):
 @pytest.mark.parametrize("offset", [0, 1, 2, 4, 8])
 @pytest.mark.parametrize("ld", [2560, 2561, 2564, 2576])
 def test_alignments_do_not_change_the_bytes(ctx, offset, ld):
-    """Every base and stride gives the bytes and scales of contiguous rows, but the norm's scales, whose sum the two forms add in
-    different orders."""
+    """Every base and stride gives the bytes and scales of contiguous rows."""
     gen = generator(ld + offset)
     t, cols = 3, 2560 - 16
     wide = randn(gen, t + 1, ld)
@@ -110,7 +109,7 @@ def test_alignments_do_not_change_the_bytes(ctx, offset, ld):
     q, untouched = guarded_rows(t, cols, offset=offset)
     before = wide.clone()
     _, s = ctx.rms_norm_s8(x, w, q, delta=delta)
-    assert torch.equal(q, q0) and torch.allclose(s, s0, rtol=2 * SCALE, atol=0)
+    assert torch.equal(q, q0) and torch.equal(s, s0)
     untouched()
     after = before.flatten().clone()
     after[offset : offset + t * ld].view(t, ld)[:, :cols] += delta
@@ -122,6 +121,39 @@ def test_alignments_do_not_change_the_bytes(ctx, offset, ld):
         _, s = ctx.quantize_tokens_s8(xk, q)
         assert torch.equal(q, q0) and torch.equal(s, s0)
         untouched()
+
+
+@pytest.mark.parametrize("rows", [1184, 1331, 4099])
+@pytest.mark.parametrize("cols", [8, 1024, 2560, 3584, 4096, 12288, 24576, 24584])
+def test_many_rows(ctx, rows, cols):
+    """Many rows (more than the blocks that are resident at once) make the bytes, scales and streams that a few rows at a time make."""
+    gen = generator(rows + cols)
+    x = randn(gen, rows, cols + 8, std=2.0)[:, :cols]
+    x[rows // 2, cols // 2] = float("nan")
+    w, smooth = randn(gen, cols, std=0.3), torch.exp(randn(gen, cols, std=0.5))
+    some = [slice(0, 700), slice(rows - 700, rows)]
+    for delta in (None, torch.float16, torch.float32):
+        d = None if delta is None else randn(gen, rows, cols).to(delta)
+        for col_scale in (None, smooth):
+            stream = x.clone()
+            q, untouched = guarded_rows(rows, cols)
+            _, s = ctx.rms_norm_s8(stream, w, q, delta=d, col_scale=col_scale)
+            untouched()
+            for part in some:
+                few = x[part].clone()
+                qf, sf = ctx.rms_norm_s8(few, w, delta=None if d is None else d[part], col_scale=col_scale)
+                assert torch.equal(q[part], qf) and torch.equal(s[part].nan_to_num(), sf.nan_to_num()) and torch.equal(stream[part].nan_to_num(), few.nan_to_num())
+            assert torch.isnan(s).nonzero().flatten().tolist() == [rows // 2]
+    for kind in (torch.float16, torch.float32):
+        xk = x.to(kind)
+        for col_scale in (None, smooth):
+            q, untouched = guarded_rows(rows, cols)
+            _, s = ctx.quantize_tokens_s8(xk, q, col_scale=col_scale)
+            untouched()
+            for part in some:
+                qf, sf = ctx.quantize_tokens_s8(xk[part], col_scale=col_scale)
+                assert torch.equal(q[part], qf) and torch.equal(s[part].nan_to_num(), sf.nan_to_num())
+    ctx.check_status()
 
 
 @pytest.mark.parametrize("cols", [256, 255])
