@@ -186,18 +186,20 @@ int32_t sepal_b200_quantize_rows_s8(const void* w, uint64_t ld_w, int8_t* q, uin
 }
 
 int32_t sepal_b200_rms_norm_s8(sepal_b200_ctx* ctx, float* x, uint64_t ld_x, const void* delta, uint64_t ld_delta, int32_t delta_half, const float* w,
-                               const float* col_scale, int8_t* q, uint64_t ld_q, float* scales, uint64_t rows, uint64_t cols, float eps, void* stream) {
+                               const float* col_scale, int8_t* q, uint64_t ld_q, float* scales, void* values, uint64_t ld_values, uint64_t rows, uint64_t cols, float eps,
+                               void* stream) {
     return guarded([&] {
         require(ctx, "ctx");
-        launch_rms_norm_s8(ctx->ctx, x, ld_x, delta, ld_delta, delta_half != 0, w, col_scale, q, ld_q, scales, rows, cols, eps, static_cast<cudaStream_t>(stream));
+        launch_rms_norm_s8(ctx->ctx, x, ld_x, delta, ld_delta, delta_half != 0, w, col_scale, q, ld_q, scales, values, ld_values, rows, cols, eps,
+                           static_cast<cudaStream_t>(stream));
     });
 }
 
 int32_t sepal_b200_quantize_tokens_s8(sepal_b200_ctx* ctx, const void* x, uint64_t ld_x, int32_t x_half, const float* col_scale, int8_t* q, uint64_t ld_q,
-                                      float* scales, uint64_t rows, uint64_t cols, void* stream) {
+                                      float* scales, void* values, uint64_t ld_values, uint64_t rows, uint64_t cols, void* stream) {
     return guarded([&] {
         require(ctx, "ctx");
-        launch_quantize_tokens_s8(ctx->ctx, x, ld_x, x_half != 0, col_scale, q, ld_q, scales, rows, cols, static_cast<cudaStream_t>(stream));
+        launch_quantize_tokens_s8(ctx->ctx, x, ld_x, x_half != 0, col_scale, q, ld_q, scales, values, ld_values, rows, cols, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -46,6 +46,8 @@ struct RowsParams {
     std::int8_t* q;
     std::size_t ld_q;
     float* scales;
+    __half* values;  // or null
+    std::size_t ld_values;
     std::size_t cols;
     float eps;
 };
@@ -99,13 +101,41 @@ __device__ __forceinline__ RowScale row_scale(float sum, unsigned top_bits, cons
 }
 
 // Round to nearest even by adding 1.5 * 2^23: |u lift inv| is at most 127 (1 + 2^-23), so the low byte of the sum is the integer in two's
-// complement. One addition where a conversion runs at a quarter of the rate.
-__device__ __forceinline__ unsigned rounded(float u, const RowScale& s) {
-    return __float_as_uint(__fadd_rn(__fmul_rn(__fmul_rn(u, s.lift), s.inv), 12582912.0f));
-}
-__device__ __forceinline__ unsigned four_bytes(float a, float b, float c, float d, const RowScale& s) {
-    if (!s.finite) return 0u;
-    return __byte_perm(__byte_perm(rounded(a, s), rounded(b, s), 0x0040), __byte_perm(rounded(c, s), rounded(d, s), 0x0040), 0x5410);
+// complement, and the sum less 1.5 * 2^23 the integer itself. One addition where a conversion runs at a quarter of the rate.
+constexpr float kRound = 12582912.0f;
+__device__ __forceinline__ float rounded(float u, const RowScale& s) { return __fadd_rn(__fmul_rn(__fmul_rn(u, s.lift), s.inv), kRound); }
+__device__ __forceinline__ unsigned byte_of(float r) { return __float_as_uint(r) & 0xFFu; }
+// What a byte stands for, in binary16: one float32 product, rounded once more.
+__device__ __forceinline__ __half value_of(float r, const RowScale& s) { return __float2half_rn(__fmul_rn(__fsub_rn(r, kRound), s.scale)); }
+
+// N consecutive results, four or eight: one store of their bytes, and one of their values where they are asked for.
+template <bool VALUES, int N>
+__device__ __forceinline__ void store_vector(const RowsParams& p, std::size_t row, unsigned vec, const float (&u)[N], const RowScale& s) {
+    unsigned bytes[N / 4], halves[N / 2];
+    if (!s.finite) {  // (the whole block's)
+#pragma unroll
+        for (int h = 0; h < N / 4; ++h) bytes[h] = 0u, halves[2 * h] = halves[2 * h + 1] = 0x7FFF7FFFu;
+    } else {
+#pragma unroll
+        for (int h = 0; h < N / 4; ++h) {
+            float r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = rounded(u[4 * h + j], s);
+            bytes[h] = __byte_perm(__byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040), __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040), 0x5410);
+            if constexpr (VALUES) {
+                const __half2 lo = __halves2half2(value_of(r[0], s), value_of(r[1], s)), hi = __halves2half2(value_of(r[2], s), value_of(r[3], s));
+                halves[2 * h] = *reinterpret_cast<const unsigned*>(&lo), halves[2 * h + 1] = *reinterpret_cast<const unsigned*>(&hi);
+            }
+        }
+    }
+    std::int8_t* const q = p.q + row * p.ld_q;
+    if constexpr (N == 8) {
+        reinterpret_cast<uint2*>(q)[vec] = make_uint2(bytes[0], bytes[1]);
+        if constexpr (VALUES) reinterpret_cast<uint4*>(p.values + row * p.ld_values)[vec] = make_uint4(halves[0], halves[1], halves[2], halves[3]);
+    } else {
+        reinterpret_cast<unsigned*>(q)[vec] = bytes[0];
+        if constexpr (VALUES) reinterpret_cast<uint2*>(p.values + row * p.ld_values)[vec] = make_uint2(halves[0], halves[1]);
+    }
 }
 
 __device__ __forceinline__ void widen(const uint4& raw, float (&v)[8]) {
@@ -140,7 +170,7 @@ __device__ __forceinline__ unsigned largest_of(unsigned top, const float4& u) {
 
 // DELTA: 0 none, 1 binary16, 2 float32. A vector is four values. WIDE: blocks of more than kNarrowThreads, held to registers that let two
 // of them onto an SM (12288 float32 values a row, 4096 rows: 63 us with one, 46 with two); narrow blocks are faster with all they ask for.
-template <int DELTA, bool WIDE>
+template <int DELTA, bool WIDE, bool VALUES>
 __global__ void __launch_bounds__(WIDE ? kMaxThreads : kNarrowThreads, WIDE ? 2 : 1) rms_norm_s8_kernel(const RowsParams p) {
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
@@ -197,15 +227,14 @@ __global__ void __launch_bounds__(WIDE ? kMaxThreads : kNarrowThreads, WIDE ? 2 
     }
     reduce_row<true>(sum, top);
     const RowScale s = row_scale<true>(sum, top, p);
-    unsigned* const out = reinterpret_cast<unsigned*>(p.q + row * p.ld_q);
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const unsigned c = threadIdx.x + blockDim.x * i;
-        if (c < vecs) out[c] = four_bytes(held[i].x, held[i].y, held[i].z, held[i].w, s);
+        if (c < vecs) store_vector<VALUES>(p, row, c, {held[i].x, held[i].y, held[i].z, held[i].w}, s);
     }
     for (unsigned c = threadIdx.x + blockDim.x * kHeld; c < vecs; c += blockDim.x) {
         const float4 u = gained(xr[c], c);  // this thread's own write, where there was one
-        out[c] = four_bytes(u.x, u.y, u.z, u.w, s);
+        store_vector<VALUES>(p, row, c, {u.x, u.y, u.z, u.w}, s);
     }
     if (threadIdx.x == 0) p.scales[row] = s.scale;
 }
@@ -226,17 +255,8 @@ __device__ __forceinline__ void row_values(const uint4& raw, const float4* smoot
         v[4 * h + 2] = __fmul_rn(v[4 * h + 2], m.z), v[4 * h + 3] = __fmul_rn(v[4 * h + 3], m.w);
     }
 }
-template <bool HALF>
-__device__ __forceinline__ void store_bytes(std::int8_t* q, unsigned c, const float (&v)[HALF ? 8 : 4], const RowScale& s) {
-    const unsigned lo = four_bytes(v[0], v[1], v[2], v[3], s);
-    if constexpr (HALF)
-        reinterpret_cast<uint2*>(q)[c] = make_uint2(lo, four_bytes(v[4], v[5], v[6], v[7], s));
-    else
-        reinterpret_cast<unsigned*>(q)[c] = lo;
-}
-
 // Quantisation alone, a block to a row; the vectors are kept as they came.
-template <bool HALF, bool WIDE>
+template <bool HALF, bool WIDE, bool VALUES>
 __global__ void __launch_bounds__(WIDE ? kMaxThreads : kNarrowThreads, WIDE ? 2 : 1) quantize_tokens_s8_kernel(const RowsParams p) {
     constexpr int kValues = HALF ? 8 : 4;
     ptx::grid_launch_dependents();
@@ -271,7 +291,7 @@ __global__ void __launch_bounds__(WIDE ? kMaxThreads : kNarrowThreads, WIDE ? 2 
     const auto store = [&](const uint4& raw, unsigned c) {
         float v[kValues];
         row_values<HALF>(raw, smooth, c, v);
-        store_bytes<HALF>(p.q + row * p.ld_q, c, v, s);
+        store_vector<VALUES>(p, row, c, v, s);
     };
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
@@ -320,8 +340,11 @@ __global__ void __launch_bounds__(kMaxThreads) rows_s8_any_kernel(const RowsPara
     const RowScale s = row_scale<NORM>(sum, top, p);
     for (std::size_t first = 4 * static_cast<std::size_t>(threadIdx.x); first < p.cols; first += 4 * static_cast<std::size_t>(blockDim.x)) {
         const std::size_t end = first + 4 < p.cols ? first + 4 : p.cols;
-        for (std::size_t c = first; c < end; ++c)
-            p.q[row * p.ld_q + c] = s.finite ? static_cast<std::int8_t>(rounded(gained(fetch(c), c), s) & 0xFFu) : std::int8_t{0};
+        for (std::size_t c = first; c < end; ++c) {
+            const float r = s.finite ? rounded(gained(fetch(c), c), s) : kRound;
+            p.q[row * p.ld_q + c] = static_cast<std::int8_t>(byte_of(r));
+            if (p.values != nullptr) p.values[row * p.ld_values + c] = value_of(r, s);
+        }
     }
     if (threadIdx.x == 0) p.scales[row] = s.scale;
 }
@@ -334,31 +357,42 @@ unsigned threads_for(std::size_t vecs) {
     return want > kMaxThreads ? kMaxThreads : static_cast<unsigned>(want);
 }
 
-void check_rows(const char* who, std::size_t rows, std::size_t cols, std::size_t ld_x, std::size_t ld_q) {
-    if (cols == 0 || ld_x < cols || ld_q < cols) throw std::invalid_argument(std::string(who) + ": a row has at least one value and the strides hold a row");
+using RowsKernel = void (*)(RowsParams);
+template <int DELTA>
+RowsKernel norm_kernel(unsigned threads, const void* values) {
+    if (threads > kNarrowThreads) return values != nullptr ? rms_norm_s8_kernel<DELTA, true, true> : rms_norm_s8_kernel<DELTA, true, false>;
+    return values != nullptr ? rms_norm_s8_kernel<DELTA, false, true> : rms_norm_s8_kernel<DELTA, false, false>;
+}
+template <bool HALF>
+RowsKernel quantise_kernel(unsigned threads, const void* values) {
+    if (threads > kNarrowThreads) return values != nullptr ? quantize_tokens_s8_kernel<HALF, true, true> : quantize_tokens_s8_kernel<HALF, true, false>;
+    return values != nullptr ? quantize_tokens_s8_kernel<HALF, false, true> : quantize_tokens_s8_kernel<HALF, false, false>;
+}
+
+void check_rows(const char* who, std::size_t rows, std::size_t cols, std::size_t ld_x, std::size_t ld_q, const void* values, std::size_t ld_values) {
+    if (cols == 0 || ld_x < cols || ld_q < cols || (values != nullptr && ld_values < cols)) throw std::invalid_argument(std::string(who) + ": a row has at least one value and the strides hold a row");
     if (rows > 0x7FFFFFFFu || cols > 0x7FFFFFFFu) throw std::invalid_argument(std::string(who) + ": dimension beyond 2^31");
 }
 
 }  // namespace
 
 void launch_rms_norm_s8(const Context& ctx, float* x, std::size_t ld_x, const void* delta, std::size_t ld_delta, bool delta_half, const float* w, const float* col_scale,
-                        std::int8_t* q, std::size_t ld_q, float* scales, std::size_t rows, std::size_t cols, float eps, cudaStream_t stream) {
-    check_rows("launch_rms_norm_s8", rows, cols, ld_x, ld_q);
+                        std::int8_t* q, std::size_t ld_q, float* scales, void* values, std::size_t ld_values, std::size_t rows, std::size_t cols, float eps, cudaStream_t stream) {
+    check_rows("launch_rms_norm_s8", rows, cols, ld_x, ld_q, values, ld_values);
     if (delta != nullptr && ld_delta < cols) throw std::invalid_argument("launch_rms_norm_s8: the stride of delta does not hold a row");
     if (!(eps >= 1.0e-30f) || !std::isfinite(eps)) throw std::invalid_argument("launch_rms_norm_s8: eps must be a positive number (1e-30 at least)");
     if (rows == 0) return;
     if (x == nullptr || w == nullptr || q == nullptr || scales == nullptr) throw std::invalid_argument("launch_rms_norm_s8: null pointer");
     check(cudaSetDevice(ctx.device), "cudaSetDevice");
-    const RowsParams p{x, ld_x, delta, ld_delta, w, col_scale, q, ld_q, scales, cols, eps};
+    const RowsParams p{x, ld_x, delta, ld_delta, w, col_scale, q, ld_q, scales, static_cast<__half*>(values), ld_values, cols, eps};
     const unsigned kind = delta == nullptr ? 0u : delta_half ? 1u : 2u;
     const bool vectors = cols % 4 == 0 && ld_x % 4 == 0 && ld_q % 4 == 0 && aligned(x, 16) && aligned(w, 16) && aligned(q, 4) &&
-                         (col_scale == nullptr || aligned(col_scale, 16)) && (kind == 0 || (ld_delta % 4 == 0 && aligned(delta, delta_half ? 8 : 16)));
+                         (col_scale == nullptr || aligned(col_scale, 16)) && (kind == 0 || (ld_delta % 4 == 0 && aligned(delta, delta_half ? 8 : 16))) && (values == nullptr || (ld_values % 4 == 0 && aligned(values, 8)));
     const dim3 grid(static_cast<unsigned>(rows));
     if (vectors) {
         const unsigned threads = threads_for(cols / 4);
-        const auto narrow = kind == 0 ? rms_norm_s8_kernel<0, false> : kind == 1 ? rms_norm_s8_kernel<1, false> : rms_norm_s8_kernel<2, false>;
-        const auto wide = kind == 0 ? rms_norm_s8_kernel<0, true> : kind == 1 ? rms_norm_s8_kernel<1, true> : rms_norm_s8_kernel<2, true>;
-        launch_kernel(threads > kNarrowThreads ? wide : narrow, grid, dim3(threads), 0, stream, "rms_norm_s8_kernel launch", p);
+        launch_kernel(kind == 0 ? norm_kernel<0>(threads, values) : kind == 1 ? norm_kernel<1>(threads, values) : norm_kernel<2>(threads, values), grid,
+                      dim3(threads), 0, stream, "rms_norm_s8_kernel launch", p);
     } else {
         const auto kernel = kind == 0 ? rows_s8_any_kernel<true, false, 0> : kind == 1 ? rows_s8_any_kernel<true, false, 1> : rows_s8_any_kernel<true, false, 2>;
         launch_kernel(kernel, grid, dim3(threads_for((cols + 3) / 4)), 0, stream, "rows_s8_any_kernel launch", p);
@@ -366,22 +400,21 @@ void launch_rms_norm_s8(const Context& ctx, float* x, std::size_t ld_x, const vo
     count_launch();
 }
 
-void launch_quantize_tokens_s8(const Context& ctx, const void* x, std::size_t ld_x, bool x_half, const float* col_scale, std::int8_t* q, std::size_t ld_q, float* scales,
+void launch_quantize_tokens_s8(const Context& ctx, const void* x, std::size_t ld_x, bool x_half, const float* col_scale, std::int8_t* q, std::size_t ld_q, float* scales, void* values, std::size_t ld_values,
                                std::size_t rows, std::size_t cols, cudaStream_t stream) {
-    check_rows("launch_quantize_tokens_s8", rows, cols, ld_x, ld_q);
+    check_rows("launch_quantize_tokens_s8", rows, cols, ld_x, ld_q, values, ld_values);
     if (rows == 0) return;
     if (x == nullptr || q == nullptr || scales == nullptr) throw std::invalid_argument("launch_quantize_tokens_s8: null pointer");
     check(cudaSetDevice(ctx.device), "cudaSetDevice");
-    const RowsParams p{x, ld_x, nullptr, 0, nullptr, col_scale, q, ld_q, scales, cols, 0.0f};
-    const std::size_t values = x_half ? 8 : 4;
-    const bool vectors = cols % values == 0 && ld_x % values == 0 && ld_q % values == 0 && aligned(x, 16) && aligned(q, values) &&
-                         (col_scale == nullptr || aligned(col_scale, 16));
+    const RowsParams p{x, ld_x, nullptr, 0, nullptr, col_scale, q, ld_q, scales, static_cast<__half*>(values), ld_values, cols, 0.0f};
+    const std::size_t per_vec = x_half ? 8 : 4;
+    const bool vectors = cols % per_vec == 0 && ld_x % per_vec == 0 && ld_q % per_vec == 0 && aligned(x, 16) && aligned(q, per_vec) &&
+                         (col_scale == nullptr || aligned(col_scale, 16)) && (values == nullptr || (ld_values % per_vec == 0 && aligned(values, 2 * per_vec)));
     const dim3 grid(static_cast<unsigned>(rows));
     if (vectors) {
-        const unsigned threads = threads_for(cols / values);
-        const auto narrow = x_half ? quantize_tokens_s8_kernel<true, false> : quantize_tokens_s8_kernel<false, false>;
-        const auto wide = x_half ? quantize_tokens_s8_kernel<true, true> : quantize_tokens_s8_kernel<false, true>;
-        launch_kernel(threads > kNarrowThreads ? wide : narrow, grid, dim3(threads), 0, stream, "quantize_tokens_s8_kernel launch", p);
+        const unsigned threads = threads_for(cols / per_vec);
+        launch_kernel(x_half ? quantise_kernel<true>(threads, values) : quantise_kernel<false>(threads, values), grid, dim3(threads), 0, stream,
+                      "quantize_tokens_s8_kernel launch", p);
     } else {
         const auto kernel = x_half ? rows_s8_any_kernel<false, true, 0> : rows_s8_any_kernel<false, false, 0>;
         launch_kernel(kernel, grid, dim3(threads_for((cols + 3) / 4)), 0, stream, "rows_s8_any_kernel launch", p);

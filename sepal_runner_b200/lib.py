@@ -46,8 +46,8 @@ SIGNATURES = {
     "sepal_b200_gemm_w8g": (_i32, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _u64, _i32, _u64, _u64, _u64, _i32, _i32, _vp]),
     "sepal_b200_gemm_w8r": (_i32, [_vp, _vp, _u64, _vp, _u64, _vp, _vp, _u64, _i32, _u64, _u64, _u64, _i32, _i32, _vp]),
     "sepal_b200_quantize_rows_s8": (_i32, [_vp, _u64, _vp, _u64, _vp, _u64, _u64, _vp, _vp]),
-    "sepal_b200_rms_norm_s8": (_i32, [_vp, _vp, _u64, _vp, _u64, _i32, _vp, _vp, _vp, _u64, _vp, _u64, _u64, C.c_float, _vp]),
-    "sepal_b200_quantize_tokens_s8": (_i32, [_vp, _vp, _u64, _i32, _vp, _vp, _u64, _vp, _u64, _u64, _vp]),
+    "sepal_b200_rms_norm_s8": (_i32, [_vp, _vp, _u64, _vp, _u64, _i32, _vp, _vp, _vp, _u64, _vp, _vp, _u64, _u64, _u64, C.c_float, _vp]),
+    "sepal_b200_quantize_tokens_s8": (_i32, [_vp, _vp, _u64, _i32, _vp, _vp, _u64, _vp, _vp, _u64, _u64, _u64, _vp]),
     "sepal_b200_gemm_s8": (_i32, [_vp, _vp, _u64, _vp, _vp, _u64, _vp, _vp, _u64, _i32, _u64, _u64, _u64, _i32, _i32, _vp]),
     "sepal_b200_quantize_group_s8": (_i32, [_vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _vp]),
     "sepal_b200_prepare_w8g_scales": (_i32, [_vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp]),
@@ -344,10 +344,18 @@ class Context:
             _require_floats(scales, t, self.device, who, "scales")
         return q, scales
 
-    def rms_norm_s8(self, x, w, q=None, scales=None, *, delta=None, col_scale=None, eps: float = 1e-6, stream=None):
+    def _values_out(self, t: int, k: int, values, who: str):
+        if values is None:
+            return None, 0
+        if values.shape != (t, k) or values.dtype is not _torch().float16 or not _rows_of(values, self.device):
+            raise ValueError(f"{who}: values must be float16 [{t}, {k}] on cuda:{self.device} with contiguous rows, not {values.dtype} {tuple(values.shape)}")
+        return values.data_ptr(), _ld(values, k)
+
+    def rms_norm_s8(self, x, w, q=None, scales=None, *, delta=None, col_scale=None, eps: float = 1e-6, values=None, stream=None):
         """The residual's addition (x += delta, in place; delta None: x is only read), the zero-centred RMSNorm and one int8 row with a
         float32 scale a token (sepal_b200_rms_norm_s8). x float32 [T, C], w float32 [C], delta float16 or float32 [T, C], col_scale float32
-        [C] (smoothing factors); returns (q int8 [T, C], scales float32 [T])."""
+        [C] (smoothing factors), values None or float16 [T, C], which gets what the bytes stand for; returns (q int8 [T, C], scales float32
+        [T])."""
         torch, device = _torch(), self.device
         if x.dim() != 2 or x.dtype is not torch.float32 or not _rows_of(x, device):
             raise ValueError(f"rms_norm_s8: x must be float32 [T, C] on cuda:{device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
@@ -361,13 +369,14 @@ class Context:
                 raise ValueError(f"rms_norm_s8: delta must be float16 or float32 {tuple(x.shape)} on cuda:{device} with contiguous rows")
             added, ld_added, half = delta.data_ptr(), _ld(delta, c), 1 if delta.dtype is torch.float16 else 0
         q, scales = self._rows_out(t, c, q, scales, "rms_norm_s8")
+        stands, ld_stands = self._values_out(t, c, values, "rms_norm_s8")
         _check(self._lib.sepal_b200_rms_norm_s8(self._h, x.data_ptr(), _ld(x, c), added, ld_added, half, w.data_ptr(), None if col_scale is None else col_scale.data_ptr(),
-                                                q.data_ptr(), _ld(q, c), scales.data_ptr(), t, c, eps, self._stream(stream)))
+                                                q.data_ptr(), _ld(q, c), scales.data_ptr(), stands, ld_stands, t, c, eps, self._stream(stream)))
         return q, scales
 
-    def quantize_tokens_s8(self, x, q=None, scales=None, *, col_scale=None, stream=None):
+    def quantize_tokens_s8(self, x, q=None, scales=None, *, col_scale=None, values=None, stream=None):
         """One int8 row with a float32 scale a token (sepal_b200_quantize_tokens_s8): x float16 or float32 [T, K] (times col_scale, float32
-        [K]); returns (q int8 [T, K], scales float32 [T])."""
+        [K]), values None or float16 [T, K], which gets what the bytes stand for; returns (q int8 [T, K], scales float32 [T])."""
         torch, device = _torch(), self.device
         if x.dim() != 2 or x.dtype not in (torch.float16, torch.float32) or not _rows_of(x, device):
             raise ValueError(f"quantize_tokens_s8: x must be float16 or float32 [T, K] on cuda:{device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
@@ -375,9 +384,10 @@ class Context:
         if col_scale is not None:
             _require_floats(col_scale, k, device, "quantize_tokens_s8", "col_scale")
         q, scales = self._rows_out(t, k, q, scales, "quantize_tokens_s8")
+        stands, ld_stands = self._values_out(t, k, values, "quantize_tokens_s8")
         _check(self._lib.sepal_b200_quantize_tokens_s8(self._h, x.data_ptr(), _ld(x, k), 1 if x.dtype is torch.float16 else 0,
                                                        None if col_scale is None else col_scale.data_ptr(), q.data_ptr(), _ld(q, k), scales.data_ptr(),
-                                                       t, k, self._stream(stream)))
+                                                       stands, ld_stands, t, k, self._stream(stream)))
         return q, scales
 
     def gemm_s8(self, xq, sx, wq, sw, y=None, *, epilogue: int = STORE, y_half: bool = True, config: int = -1, stream=None):

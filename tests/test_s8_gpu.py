@@ -36,6 +36,14 @@ def check_rows(q, scales, v):
     assert q.abs().max() <= 127
 
 
+def check_values(buffer, q, scales):
+    """The binary16 values of the bytes, to the bit, inside a buffer of nines."""
+    t, c = q.shape
+    want = torch.full_like(buffer, 9.0)
+    want[1 : t + 1, :c] = (q.float() * scales[:, None]).half()
+    assert torch.equal(buffer.nan_to_num(3.0), want.nan_to_num(3.0))
+
+
 def guarded_rows(t, c, pad=16, offset=0):
     """int8 rows of c values inside a buffer of 99s, and a check that nothing else of it was written."""
     ld = (c + 15) // 16 * 16 + pad
@@ -68,8 +76,10 @@ def test_norm(ctx, cols, delta):
         stream = x.clone()
         q, untouched = guarded_rows(t, cols)
         scales = torch.full((t + 2,), 7.0, device="cuda")
-        ctx.rms_norm_s8(stream, w, q, scales[1 : t + 1], delta=d, col_scale=col_scale, eps=1e-6)
+        values = torch.full((t + 2, cols + 4), 9.0, device="cuda").half()
+        ctx.rms_norm_s8(stream, w, q, scales[1 : t + 1], delta=d, col_scale=col_scale, eps=1e-6, values=values[1 : t + 1, :cols])
         assert torch.equal(stream, want_x)
+        check_values(values, q, scales[1 : t + 1])
         v = want_x.double()
         v = v / (v.square().mean(1, keepdim=True) + 1e-6).sqrt() * (1 + w.double())
         check_rows(q, scales[1 : t + 1], v if col_scale is None else v * smooth.double())
@@ -86,7 +96,9 @@ def test_quantiser(ctx, cols, half):
     smooth = torch.exp(randn(gen, cols, std=0.5))
     for col_scale in (None, smooth):
         q, untouched = guarded_rows(t, cols)
-        _, scales = ctx.quantize_tokens_s8(x, q, col_scale=col_scale)
+        values = torch.full((t + 2, cols + 4), 9.0, device="cuda").half()
+        _, scales = ctx.quantize_tokens_s8(x, q, col_scale=col_scale, values=values[1 : t + 1, :cols])
+        check_values(values, q, scales)
         check_rows(q, scales, x.double() if col_scale is None else x.double() * smooth.double())
         untouched()
         if half and cols % 16 == 0:
@@ -172,7 +184,9 @@ def test_rows_that_are_zero_tiny_huge_or_not_finite(ctx, cols):
     x[7, 0] = -inf
     x[8, 5], x[8, 6] = inf, nan
     w = torch.zeros(cols, device="cuda")
-    q, s = ctx.quantize_tokens_s8(x)
+    values = torch.full((12, cols + 4), 9.0, device="cuda").half()
+    q, s = ctx.quantize_tokens_s8(x, values=values[1:11, :cols])
+    check_values(values, q, s)
     for r in (0, 9):
         assert torch.equal(q[r], plain_q[r]) and s[r] == plain_s[r]
     check_rows(q[1:5], s[1:5], x[1:5].double())
@@ -471,8 +485,8 @@ def test_refusals_of_the_library(ctx):
     q = torch.zeros((4, 64), dtype=torch.int8, device="cuda")
     s, y = torch.zeros(64, device="cuda"), torch.full((4, 128), 5.0, device="cuda")
 
-    def norm(ld_x=64, delta=None, ld_delta=64, w=s, ld_q=64, cols=64, eps=1e-6, rows=4):
-        return lib.sepal_b200_rms_norm_s8(h, x.data_ptr(), ld_x, delta, ld_delta, 0, None if w is None else w.data_ptr(), None, q.data_ptr(), ld_q, s.data_ptr(), rows, cols,
+    def norm(ld_x=64, delta=None, ld_delta=64, w=s, ld_q=64, cols=64, eps=1e-6, rows=4, values=None, ld_values=0):
+        return lib.sepal_b200_rms_norm_s8(h, x.data_ptr(), ld_x, delta, ld_delta, 0, None if w is None else w.data_ptr(), None, q.data_ptr(), ld_q, s.data_ptr(), values, ld_values, rows, cols,
                                           eps, None)
 
     def multiply(xq=None, ld_x=64, ld_w=64, ld_y=64, n=64, k=64, epilogue=0, config=-1, t=4, sx=s):
@@ -480,7 +494,7 @@ def test_refusals_of_the_library(ctx):
                                       ld_y, 0, t, n, k, epilogue, config, None)
 
     for call in (lambda: norm(ld_x=63), lambda: norm(ld_q=63), lambda: norm(delta=x.data_ptr(), ld_delta=63), lambda: norm(w=None), lambda: norm(cols=0),
-                 lambda: norm(ld_x=0), lambda: norm(eps=0.0), lambda: norm(eps=-1.0), lambda: norm(eps=float("nan")), lambda: norm(eps=float("inf")), lambda: norm(rows=1 << 31),
+                 lambda: norm(ld_x=0), lambda: norm(values=y.data_ptr(), ld_values=63), lambda: norm(eps=0.0), lambda: norm(eps=-1.0), lambda: norm(eps=float("nan")), lambda: norm(eps=float("inf")), lambda: norm(rows=1 << 31),
                  lambda: multiply(ld_x=72), lambda: multiply(ld_x=48), lambda: multiply(ld_w=72), lambda: multiply(ld_y=63), lambda: multiply(k=0),
                  lambda: multiply(n=0), lambda: multiply(k=1 << 17, ld_x=1 << 17, ld_w=1 << 17), lambda: multiply(epilogue=2), lambda: multiply(epilogue=3),
                  lambda: multiply(xq=q.data_ptr() + 8), lambda: multiply(sx=None), lambda: multiply(config=0), lambda: multiply(config=-2), lambda: multiply(config=512),
@@ -492,6 +506,6 @@ def test_refusals_of_the_library(ctx):
     assert lib.sepal_b200_status(h, None, C.byref(out)) == 0 and out.value == 0
     assert (y == 5).all() and (q == 0).all()
     # nothing to do is no error, whatever the pointers
-    assert lib.sepal_b200_rms_norm_s8(h, None, 64, None, 0, 0, None, None, None, 64, None, 0, 64, 1e-6, None) == 0
-    assert lib.sepal_b200_quantize_tokens_s8(h, None, 64, 1, None, None, 64, None, 0, 64, None) == 0
+    assert lib.sepal_b200_rms_norm_s8(h, None, 64, None, 0, 0, None, None, None, 64, None, None, 0, 0, 64, 1e-6, None) == 0
+    assert lib.sepal_b200_quantize_tokens_s8(h, None, 64, 1, None, None, 64, None, None, 0, 0, 64, None) == 0
     assert lib.sepal_b200_gemm_s8(h, None, 64, None, None, 64, None, None, 64, 0, 0, 64, 64, 0, -1, None) == 0
