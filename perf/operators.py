@@ -136,12 +136,12 @@ def run(state):
         return _run_gemm(state)
     if own:
         _, ctx = _context()
+        # the values that the bytes stand for come from the same call
         if state["kind"] == "norm":
-            ctx.rms_norm_s8(state["x"], state["w"], state["q"], state["scales"], delta=state["delta"], col_scale=state["smooth"], eps=EPS)
+            ctx.rms_norm_s8(state["x"], state["w"], state["q"], state["scales"], delta=state["delta"], col_scale=state["smooth"], eps=EPS, values=state["values"])
         else:
-            ctx.quantize_tokens_s8(state["x"], state["q"], state["scales"], col_scale=state["smooth"])
-        # the values that the bytes stand for
-        out = {"values": torch.mul(state["q"], state["by_row"], out=state["values"]), "scales": state["scales"]}
+            ctx.quantize_tokens_s8(state["x"], state["q"], state["scales"], col_scale=state["smooth"], values=state["values"])
+        out = {"values": state["values"], "scales": state["scales"]}
     else:
         x = state["x"]
         if state["kind"] == "norm":
