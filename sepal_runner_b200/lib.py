@@ -145,19 +145,28 @@ def _torch():
     return _TORCH
 
 
-def _rows_of(t, device: int) -> bool:
-    """Whether t lies on cuda:`device` and its rows are contiguous. (get_device: a number, where t.device builds an object.)"""
-    return t.get_device() == device and (t.stride(-1) == 1 or t.shape[-1] == 1 or t.numel() == 0)
+def _matrix(t, dtypes, device: int):
+    """(rows, columns, row stride) of a matrix of one of `dtypes` on cuda:`device` whose rows are contiguous, or None. A lone row's stride, to
+    which torch may give any value, is said to be its length. (Few and cheap questions: at one token a call's checks are what it costs.)"""
+    if t.dtype not in dtypes or t.get_device() != device:
+        return None
+    shape = t.shape
+    if len(shape) != 2:
+        return None
+    rows, columns = shape
+    ld, step = t.stride()
+    if step != 1 and columns > 1 and rows > 0:
+        return None
+    return rows, columns, ld if rows > 1 else columns
 
 
-def _ld(t, row: int) -> int:
-    """The row stride of a matrix in elements; `row` where it has one row or none (a stride torch may give any value)."""
-    return t.stride(0) if t.shape[0] > 1 else row
+def _vector(t, n: int, device: int) -> bool:
+    """Whether t is n contiguous float32 values on cuda:`device`."""
+    return t.dtype is _TORCH.float32 and t.get_device() == device and t.numel() == n and t.is_contiguous()
 
 
-def _require_floats(t, n: int, device: int, who: str, what: str) -> None:
-    if t.dtype is not _torch().float32 or t.numel() != n or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{who}: {what} must be {n} contiguous float32 values on cuda:{device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+def _wanted(who: str, what: str, kinds: str, device: int, t) -> str:
+    return f"{who}: {what} must be {kinds} on cuda:{device} with contiguous rows, not {t.dtype} {tuple(t.shape)} of stride {t.stride()} on {t.device}"
 
 
 @dataclass
@@ -329,27 +338,37 @@ class Context:
         """The cudaStream_t of `stream`, or of the current stream of the context's device (which need not be the current one)."""
         if stream is not None:
             return int(stream.cuda_stream)
-        raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
-        return int(_torch().cuda.current_stream(self.device).cuda_stream) if raw is None else raw(self.device)
+        raw = getattr(_TORCH._C, "_cuda_getCurrentRawStream", None)
+        return int(_TORCH.cuda.current_stream(self.device).cuda_stream) if raw is None else raw(self.device)
 
-    def _rows_out(self, t: int, k: int, q, scales, who: str):
-        """The int8 rows and their scales: new ones (rows of a multiple of 16 bytes, as gemm_s8 takes them), or the caller's after checks."""
+    def _row_operands(self, who: str, t: int, c: int, q, scales, col_scale, values):
+        """What the two calls that leave int8 rows have in common: q and scales (new ones, q in rows of a multiple of 16 bytes as gemm_s8 takes
+        them, or the caller's after checks), and the pointers and strides of q, scales, col_scale and values."""
+        torch, device = _TORCH, self.device
         if q is None:
-            q = _torch().empty((t, (k + 15) // 16 * 16), dtype=_torch().int8, device=f"cuda:{self.device}")[:, :k]
-        elif q.shape != (t, k) or q.dtype is not _torch().int8 or not _rows_of(q, self.device):
-            raise ValueError(f"{who}: q must be int8 [{t}, {k}] on cuda:{self.device} with contiguous rows, not {q.dtype} {tuple(q.shape)}")
-        if scales is None:
-            scales = _torch().empty((t,), dtype=_torch().float32, device=f"cuda:{self.device}")
+            ld_q = (c + 15) // 16 * 16
+            q = torch.empty((t, ld_q), dtype=torch.int8, device=f"cuda:{device}")[:, :c]
         else:
-            _require_floats(scales, t, self.device, who, "scales")
-        return q, scales
-
-    def _values_out(self, t: int, k: int, values, who: str):
-        if values is None:
-            return None, 0
-        if values.shape != (t, k) or values.dtype is not _torch().float16 or not _rows_of(values, self.device):
-            raise ValueError(f"{who}: values must be float16 [{t}, {k}] on cuda:{self.device} with contiguous rows, not {values.dtype} {tuple(values.shape)}")
-        return values.data_ptr(), _ld(values, k)
+            got = _matrix(q, (torch.int8,), device)
+            if got is None or got[0] != t or got[1] != c:
+                raise ValueError(_wanted(who, "q", f"int8 [{t}, {c}]", device, q))
+            ld_q = got[2]
+        if scales is None:
+            scales = torch.empty((t,), dtype=torch.float32, device=f"cuda:{device}")
+        elif not _vector(scales, t, device):
+            raise ValueError(_wanted(who, "scales", f"{t} float32 values", device, scales))
+        smooth = stands = None
+        ld_stands = 0
+        if col_scale is not None:
+            if not _vector(col_scale, c, device):
+                raise ValueError(_wanted(who, "col_scale", f"{c} float32 values", device, col_scale))
+            smooth = col_scale.data_ptr()
+        if values is not None:
+            got = _matrix(values, (torch.float16,), device)
+            if got is None or got[0] != t or got[1] != c:
+                raise ValueError(_wanted(who, "values", f"float16 [{t}, {c}]", device, values))
+            stands, ld_stands = values.data_ptr(), got[2]
+        return q, scales, (smooth, q.data_ptr(), ld_q, scales.data_ptr(), stands, ld_stands)
 
     def rms_norm_s8(self, x, w, q=None, scales=None, *, delta=None, col_scale=None, eps: float = 1e-6, values=None, stream=None):
         """The residual's addition (x += delta, in place; delta None: x is only read), the zero-centred RMSNorm and one int8 row with a
@@ -357,63 +376,65 @@ class Context:
         [C] (smoothing factors), values None or float16 [T, C], which gets what the bytes stand for; returns (q int8 [T, C], scales float32
         [T])."""
         torch, device = _torch(), self.device
-        if x.dim() != 2 or x.dtype is not torch.float32 or not _rows_of(x, device):
-            raise ValueError(f"rms_norm_s8: x must be float32 [T, C] on cuda:{device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
-        t, c = x.shape
-        _require_floats(w, c, device, "rms_norm_s8", "w")
-        if col_scale is not None:
-            _require_floats(col_scale, c, device, "rms_norm_s8", "col_scale")
+        got = _matrix(x, (torch.float32,), device)
+        if got is None:
+            raise ValueError(_wanted("rms_norm_s8", "x", "float32 [T, C]", device, x))
+        t, c, ld_x = got
+        if not _vector(w, c, device):
+            raise ValueError(_wanted("rms_norm_s8", "w", f"{c} float32 values", device, w))
         added, ld_added, half = None, 0, 0
         if delta is not None:
-            if delta.shape != x.shape or delta.dtype not in (torch.float16, torch.float32) or not _rows_of(delta, device):
-                raise ValueError(f"rms_norm_s8: delta must be float16 or float32 {tuple(x.shape)} on cuda:{device} with contiguous rows")
-            added, ld_added, half = delta.data_ptr(), _ld(delta, c), 1 if delta.dtype is torch.float16 else 0
-        q, scales = self._rows_out(t, c, q, scales, "rms_norm_s8")
-        stands, ld_stands = self._values_out(t, c, values, "rms_norm_s8")
-        _check(self._lib.sepal_b200_rms_norm_s8(self._h, x.data_ptr(), _ld(x, c), added, ld_added, half, w.data_ptr(), None if col_scale is None else col_scale.data_ptr(),
-                                                q.data_ptr(), _ld(q, c), scales.data_ptr(), stands, ld_stands, t, c, eps, self._stream(stream)))
+            got = _matrix(delta, (torch.float16, torch.float32), device)
+            if got is None or got[0] != t or got[1] != c:
+                raise ValueError(_wanted("rms_norm_s8", "delta", f"float16 or float32 [{t}, {c}]", device, delta))
+            added, ld_added, half = delta.data_ptr(), got[2], 1 if delta.dtype is torch.float16 else 0
+        q, scales, rest = self._row_operands("rms_norm_s8", t, c, q, scales, col_scale, values)
+        _check(self._lib.sepal_b200_rms_norm_s8(self._h, x.data_ptr(), ld_x, added, ld_added, half, w.data_ptr(), *rest, t, c, eps, self._stream(stream)))
         return q, scales
 
     def quantize_tokens_s8(self, x, q=None, scales=None, *, col_scale=None, values=None, stream=None):
         """One int8 row with a float32 scale a token (sepal_b200_quantize_tokens_s8): x float16 or float32 [T, K] (times col_scale, float32
         [K]), values None or float16 [T, K], which gets what the bytes stand for; returns (q int8 [T, K], scales float32 [T])."""
         torch, device = _torch(), self.device
-        if x.dim() != 2 or x.dtype not in (torch.float16, torch.float32) or not _rows_of(x, device):
-            raise ValueError(f"quantize_tokens_s8: x must be float16 or float32 [T, K] on cuda:{device} with contiguous rows, not {x.dtype} {tuple(x.shape)}")
-        t, k = x.shape
-        if col_scale is not None:
-            _require_floats(col_scale, k, device, "quantize_tokens_s8", "col_scale")
-        q, scales = self._rows_out(t, k, q, scales, "quantize_tokens_s8")
-        stands, ld_stands = self._values_out(t, k, values, "quantize_tokens_s8")
-        _check(self._lib.sepal_b200_quantize_tokens_s8(self._h, x.data_ptr(), _ld(x, k), 1 if x.dtype is torch.float16 else 0,
-                                                       None if col_scale is None else col_scale.data_ptr(), q.data_ptr(), _ld(q, k), scales.data_ptr(),
-                                                       stands, ld_stands, t, k, self._stream(stream)))
+        got = _matrix(x, (torch.float16, torch.float32), device)
+        if got is None:
+            raise ValueError(_wanted("quantize_tokens_s8", "x", "float16 or float32 [T, K]", device, x))
+        t, k, ld_x = got
+        q, scales, rest = self._row_operands("quantize_tokens_s8", t, k, q, scales, col_scale, values)
+        _check(self._lib.sepal_b200_quantize_tokens_s8(self._h, x.data_ptr(), ld_x, 1 if x.dtype is torch.float16 else 0, *rest, t, k, self._stream(stream)))
         return q, scales
 
     def gemm_s8(self, xq, sx, wq, sw, y=None, *, epilogue: int = STORE, y_half: bool = True, config: int = -1, stream=None):
         """y = epilogue(float(xq @ wq.T) * sx[:, None] * sw): xq int8 [T, K] with sx float32 [T] (rms_norm_s8, quantize_tokens_s8), wq int8
         [N, K] with sw float32 [N] (quantize_rows_s8). The sums are exact integers (sepal_b200_gemm_s8)."""
         torch, device = _torch(), self.device
-        if xq.dim() != 2 or wq.dim() != 2 or xq.dtype is not torch.int8 or wq.dtype is not torch.int8 or not _rows_of(xq, device) or not _rows_of(wq, device):
-            raise ValueError(f"gemm_s8: xq and wq must be int8 matrices on cuda:{device} with contiguous rows")
-        t, k = xq.shape
-        n, wk = wq.shape
+        got, weights = _matrix(xq, (torch.int8,), device), _matrix(wq, (torch.int8,), device)
+        if got is None:
+            raise ValueError(_wanted("gemm_s8", "xq", "int8 [T, K]", device, xq))
+        if weights is None:
+            raise ValueError(_wanted("gemm_s8", "wq", "int8 [N, K]", device, wq))
+        t, k, ld_x = got
+        n, wk, ld_w = weights
         if wk != k:
-            raise ValueError(f"gemm_s8: xq is [{t}, {k}] but wq is {tuple(wq.shape)}: the inner dimensions must agree")
-        _require_floats(sx, t, device, "gemm_s8", "sx")
-        _require_floats(sw, n, device, "gemm_s8", "sw")
+            raise ValueError(f"gemm_s8: xq is [{t}, {k}] but wq is [{n}, {wk}]: the inner dimensions must agree")
+        if not _vector(sx, t, device):
+            raise ValueError(_wanted("gemm_s8", "sx", f"{t} float32 values", device, sx))
+        if not _vector(sw, n, device):
+            raise ValueError(_wanted("gemm_s8", "sw", f"{n} float32 values", device, sw))
         columns = n // 2 if epilogue == SWIGLU else n
         if y is None:
             if epilogue == ADD:
                 raise ValueError("gemm_s8: epilogue ADD updates an output that the caller gives")
-            y = torch.empty((t, columns), dtype=torch.float16 if y_half else torch.float32, device=xq.device)
+            y, ld_y = torch.empty((t, columns), dtype=torch.float16 if y_half else torch.float32, device=xq.device), columns
         else:
-            y_half = y.dtype is torch.float16
-            if y.shape != (t, columns) or not (y_half or y.dtype is torch.float32) or not _rows_of(y, device):
-                raise ValueError(f"gemm_s8: the output must be float16 or float32 [{t}, {columns}] on cuda:{device} with contiguous rows, not {y.dtype} {tuple(y.shape)}")
-        row = (k + 15) // 16 * 16  # (a lone row's stride is never used: one that the kernels take)
-        _check(self._lib.sepal_b200_gemm_s8(self._h, xq.data_ptr(), _ld(xq, row), sx.data_ptr(), wq.data_ptr(), _ld(wq, row), sw.data_ptr(), y.data_ptr(),
-                                            _ld(y, columns), 1 if y_half else 0, t, n, k, epilogue, config, self._stream(stream)))
+            got = _matrix(y, (torch.float16, torch.float32), device)
+            if got is None or got[0] != t or got[1] != columns:
+                raise ValueError(_wanted("gemm_s8", "the output", f"float16 or float32 [{t}, {columns}]", device, y))
+            y_half, ld_y = y.dtype is torch.float16, got[2]
+        # (a lone row's stride is never used: one that the kernels take)
+        _check(self._lib.sepal_b200_gemm_s8(self._h, xq.data_ptr(), ld_x if t > 1 else (k + 15) // 16 * 16, sx.data_ptr(), wq.data_ptr(),
+                                            ld_w if n > 1 else (k + 15) // 16 * 16, sw.data_ptr(), y.data_ptr(), ld_y, 1 if y_half else 0, t, n, k, epilogue,
+                                            config, self._stream(stream)))
         return y
 
     def pack_gate_up(self, stacked, stream=None):
