@@ -261,7 +261,8 @@ typedef struct sepal_b200_trunk_config {
     uint32_t attn_q, attn_kv;             /* q width; k and v width each (one fused [q; k; v] multiply) */
     uint32_t dn_in, dn_v_offset, dn_v;    /* fused DeltaNet in-projection width; the band its out-projection reads */
     uint32_t max_call_tokens;             /* rows per call; a longer request is cut into calls (gpu_decision_engine.cpp:233-245) */
-    uint32_t mlp_int8;                    /* 1: gate_up and down stored as int8 groups */
+    uint32_t mlp_int8;                    /* 1: gate_up and down stored as int8 groups; 2: as int8 with one scale an output row, multiplied by
+                                           * int8 activations with one scale a token (the calls under "activations in 8 bits") */
     float eps;
     uint64_t seed;
     uint32_t attn_o;                      /* width the attention out-projection reads; 0: attn_q (a real q_proj also carries the output gate) */
@@ -370,7 +371,8 @@ SEPAL_B200_API int32_t sepal_b200_tensor_file_write(const char* path, uint64_t n
 
 /* The trunk with the weights of a checkpoint instead of random ones: the reference's placement (runner/cuda/src/cuda_engine.cpp:525-711)
  * for the projections this path has: [q; k; v] and [qkv; z; b; a] stacked, everything converted to binary16 (norms float32), [gate; up]
- * interleaved in blocks of 64 rows, the MLP quantised per group of 128 from a float32 copy when mlp_int8 is set. The configuration must
+ * interleaved in blocks of 64 rows, the MLP quantised per group of 128 from a float32 copy when mlp_int8 is 1 and per row of its
+ * binary16 form when it is 2. The configuration must
  * agree with the tensors' shapes (attn_q = rows of q_proj, attn_o = columns of o_proj, dn_in = rows of the four in-projections together).
  * A file written by sepal_b200_trunk_save (metadata format = "sepal_b200.placed.1") is copied to the device as it is. */
 SEPAL_B200_API int32_t sepal_b200_trunk_open_checkpoint(int32_t device, const sepal_b200_trunk_config* config, const sepal_b200_checkpoint* checkpoint,
@@ -404,7 +406,7 @@ SEPAL_B200_API int32_t sepal_b200_trunk_score(sepal_b200_trunk* trunk, uint64_t 
 /* Copies a stored weight to the host (size-query protocol: host_out NULL only reports *needed). which: 0 embedding, 1 input norm,
  * 2 mixer in-projection, 3 mixer out-projection, 4 post norm, 5 packed [gate; up], 6 down, 7 / 8 the attention core's q / k head norms,
  * 9 .. 12 the DeltaNet core's convolution, A_log, dt_bias and norm weight, 13 / 14 (int8 MLP only) the group quantiser's float32 scales of
- * [gate; up] and down, [rows, k / 128]. */
+ * [gate; up] and down, [rows, k / 128] (mlp_int8 2: the row quantiser's, [rows]). */
 SEPAL_B200_API int32_t sepal_b200_trunk_weight(sepal_b200_trunk* trunk, uint32_t layer, int32_t which, void* host_out, uint64_t capacity,
                                                uint64_t* needed);
 SEPAL_B200_API int32_t sepal_b200_trunk_info(sepal_b200_trunk* trunk, uint64_t* gemm_flops_per_token, uint64_t* weight_bytes);

@@ -167,6 +167,22 @@ void Trunk::prepare_mlp_scales(Layer& L) {
     L.down_q = prepare(L.down_scales, H, I, static_cast<const std::int8_t*>(L.down));
 }
 
+// mlp_int8 2: the MLP's matrices as bytes with one float32 scale a row, the layout of launch_gemm_s8.
+void Trunk::allocate_mlp_rows(Layer& L) {
+    const std::size_t H = cfg_.hidden, I = cfg_.intermediate;
+    L.gate_up = alloc(2 * I * H);
+    L.down = alloc(H * I);
+    L.gate_up_scales = static_cast<float*>(alloc(2 * I * 4));
+    L.down_scales = static_cast<float*>(alloc(H * 4));
+    weight_bytes_ += 3 * I * H + (2 * I + H) * 4;
+}
+// ... quantised from binary16 matrices, [gate; up] interleaved; either may be null (not yet there).
+void Trunk::place_mlp_rows(Layer& L, const void* gate_up_half, const void* down_half) {
+    const std::size_t H = cfg_.hidden, I = cfg_.intermediate;
+    if (gate_up_half != nullptr) launch_quantize_rows_s8(gate_up_half, H, static_cast<std::int8_t*>(L.gate_up), H, L.gate_up_scales, 2 * I, H, nullptr, stream_);
+    if (down_half != nullptr) launch_quantize_rows_s8(down_half, I, static_cast<std::int8_t*>(L.down), I, L.down_scales, H, I, nullptr, stream_);
+}
+
 void Trunk::place_random() {
     const TrunkConfig& c = cfg_;
     const std::size_t H = c.hidden, I = c.intermediate;
@@ -183,7 +199,7 @@ void Trunk::place_random() {
     void* packed = nullptr;
     check(cudaMalloc(&stacked, 2 * I * H * 2), "cudaMalloc(scratch)");
     if (c.mlp_int8) {
-        check(cudaMalloc(reinterpret_cast<void**>(&wide), 2 * I * H * 4), "cudaMalloc(scratch)");
+        if (!mlp_s8()) check(cudaMalloc(reinterpret_cast<void**>(&wide), 2 * I * H * 4), "cudaMalloc(scratch)");
         check(cudaMalloc(&packed, 2 * I * H * 2), "cudaMalloc(scratch)");
     }
     for (std::uint32_t l = 0; l < c.layers; ++l) {
@@ -231,6 +247,12 @@ void Trunk::place_random() {
             L.down = alloc(H * I * 2);
             fill_half(L.down, H * I);
             weight_bytes_ += (2 * I * H + H * I) * 2;
+        } else if (mlp_s8()) {
+            allocate_mlp_rows(L);
+            launch_pack_gate_up(stacked, H * 2, packed, H * 2, I, H * 2, stream_);
+            place_mlp_rows(L, packed, nullptr);
+            fill_half(stacked, H * I);
+            place_mlp_rows(L, nullptr, stacked);
         } else {
             // pack in binary16, widen, quantise per group of 128 (runner/cuda/src/cuda_engine.cpp:580-627), prepare the scales
             launch_pack_gate_up(stacked, H * 2, packed, H * 2, I, H * 2, stream_);
@@ -281,10 +303,11 @@ void Trunk::place_checkpoint(const Checkpoint& ck) {
 
     void* stacked = nullptr;  // [gate; up] before the interleave, in the type it is interleaved in
     void* packed = nullptr;
-    const std::size_t mlp_elem = c.mlp_int8 ? 4 : 2;
+    const bool groups = c.mlp_int8 != 0 && !mlp_s8();  // the group quantiser reads float32, the row quantiser binary16
+    const std::size_t mlp_elem = groups ? 4 : 2;
     check(cudaMalloc(&stacked, 2 * I * H * mlp_elem), "cudaMalloc(scratch)");
-    if (c.mlp_int8) check(cudaMalloc(&packed, 2 * I * H * 4), "cudaMalloc(scratch)");
-    const ElementType mlp_land = c.mlp_int8 ? ElementType::F32 : ElementType::F16;
+    if (c.mlp_int8) check(cudaMalloc(&packed, 2 * I * H * mlp_elem), "cudaMalloc(scratch)");
+    const ElementType mlp_land = groups ? ElementType::F32 : ElementType::F16;
 
     for (std::uint32_t l = 0; l < c.layers; ++l) {
         Layer& L = layers_[l];
@@ -340,6 +363,12 @@ void Trunk::place_checkpoint(const Checkpoint& ck) {
             L.down = alloc(H * I * 2);
             up.put(down, ElementType::F16, L.down);
             weight_bytes_ += (2 * I * H + H * I) * 2;
+        } else if (mlp_s8()) {
+            allocate_mlp_rows(L);
+            launch_pack_gate_up(stacked, H * 2, packed, H * 2, I, H * 2, stream_);
+            place_mlp_rows(L, packed, nullptr);
+            up.put(down, ElementType::F16, stacked);
+            place_mlp_rows(L, nullptr, stacked);
         } else {
             // the quantiser reads a float32 copy of the stored weights, interleaved first (runner/cuda/src/cuda_engine.cpp:580-627)
             launch_pack_gate_up(stacked, H * 4, packed, H * 4, I, H * 4, stream_);
@@ -409,6 +438,12 @@ void Trunk::place_saved(const Checkpoint& ck) {
             up.put(same_type(need(ck, pre + "gate_up", 2 * I, H), ElementType::F16), ElementType::F16, L.gate_up);
             up.put(same_type(need(ck, pre + "down", H, I), ElementType::F16), ElementType::F16, L.down);
             weight_bytes_ += (2 * I * H + H * I) * 2;
+        } else if (mlp_s8()) {
+            allocate_mlp_rows(L);
+            up.put(same_type(need(ck, pre + "gate_up", 2 * I, H), ElementType::I8), ElementType::I8, L.gate_up);
+            up.put(same_type(need(ck, pre + "down", H, I), ElementType::I8), ElementType::I8, L.down);
+            up.put(same_type(need(ck, pre + "gate_up.scales", 2 * I, 0), ElementType::F32), ElementType::F32, L.gate_up_scales);
+            up.put(same_type(need(ck, pre + "down.scales", H, 0), ElementType::F32), ElementType::F32, L.down_scales);
         } else {
             L.gate_up = alloc(2 * I * H);
             L.down = alloc(H * I);
@@ -461,10 +496,11 @@ void Trunk::save(const std::string& path) {
             add(pre + "gate_up", ElementType::F16, {2 * I, H}, L.gate_up);
             add(pre + "down", ElementType::F16, {H, I}, L.down);
         } else {
+            const auto scales = [&](std::uint64_t rows, std::uint64_t k) { return mlp_s8() ? std::vector<std::uint64_t>{rows} : std::vector<std::uint64_t>{rows, k / kGroup}; };
             add(pre + "gate_up", ElementType::I8, {2 * I, H}, L.gate_up);
-            add(pre + "gate_up.scales", ElementType::F32, {2 * I, H / kGroup}, L.gate_up_scales);
+            add(pre + "gate_up.scales", ElementType::F32, scales(2 * I, H), L.gate_up_scales);
             add(pre + "down", ElementType::I8, {H, I}, L.down);
-            add(pre + "down.scales", ElementType::F32, {H, I / kGroup}, L.down_scales);
+            add(pre + "down.scales", ElementType::F32, scales(H, I), L.down_scales);
         }
     }
     for (std::size_t i = 0; i < out.size(); ++i) out[i].data = held[i].data();  // the vectors no longer move

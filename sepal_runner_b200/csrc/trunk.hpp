@@ -34,7 +34,7 @@ struct TrunkConfig {
     std::uint32_t attn_q = 4096, attn_kv = 1024;           // q width; k and v width each
     std::uint32_t dn_in = 8192, dn_v_offset = 4096, dn_v = 2048;  // fused in-projection width; the band the out-projection reads
     std::uint32_t max_call_tokens = 4096;
-    std::uint32_t mlp_int8 = 0;                             // 1: gate_up and down stored as int8 groups
+    std::uint32_t mlp_int8 = 0;                             // 1: gate_up and down stored as int8 groups; 2: as int8 with a scale a row, activations in int8 too
     float eps = 1e-6f;
     std::uint64_t seed = 1;
     std::uint32_t attn_o = 0;                               // width the attention out-projection reads (0: attn_q); q_proj may carry a gate
@@ -52,7 +52,7 @@ struct TrunkConfig {
 extern const char* const kSavedFormat;
 
 enum class TrunkWeight : int { Embedding = 0, NormIn = 1, MixIn = 2, MixOut = 3, NormPost = 4, GateUp = 5, Down = 6, QNorm = 7, KNorm = 8, DnConv = 9, DnALog = 10, DnDtBias = 11, DnNorm = 12,
-                               GateUpScales = 13, DownScales = 14 };  // mlp_int8: the quantiser's float32 scales, [rows, k / 128]
+                               GateUpScales = 13, DownScales = 14 };  // mlp_int8: the quantiser's float32 scales, [rows, k / 128] (2: [rows])
 
 class Trunk {
 public:
@@ -112,7 +112,7 @@ private:
         float* dn_tails = nullptr;    // [slots, taps - 1, conv_dim]
         void* k_cache = nullptr;  // binary16 [arena tokens, kv width]: the keys (normed, rotated) and values of the requests being served
         void* v_cache = nullptr;
-        float* gate_up_scales = nullptr;  // mlp_int8: the quantiser's float32 scales [2 I, hidden / 128] and [hidden, I / 128]
+        float* gate_up_scales = nullptr;  // mlp_int8: the quantiser's float32 scales [2 I, hidden / 128] and [hidden, I / 128] (2: [2 I] and [hidden])
         float* down_scales = nullptr;
     };
     void* alloc(std::size_t bytes);
@@ -121,11 +121,14 @@ private:
     void place_saved(const Checkpoint& checkpoint);
     void shape_layer(std::uint32_t l);
     void prepare_mlp_scales(Layer& L);
+    void place_mlp_rows(Layer& L, const void* gate_up_half, const void* down_half);
+    void allocate_mlp_rows(Layer& L);
     void forward_call(const std::uint32_t* tokens_dev, std::size_t rows, const std::vector<AttentionRow>& runs, const std::vector<DeltaNetRow>& dn_runs);
     void reserve_cache(std::size_t tokens);
     void reserve_states(std::size_t slots);
     bool real_attention() const { return cfg_.attn_heads != 0; }
     bool real_deltanet() const { return cfg_.dn_value_heads != 0; }
+    bool mlp_s8() const { return cfg_.mlp_int8 == 2; }  // int8 activations and int8 weights, integer products
     DeltaNetShape deltanet_shape() const;
 
     TrunkConfig cfg_;
@@ -139,6 +142,10 @@ private:
     void* a1_ = nullptr;         // binary16 [max_call_tokens, hidden]
     void* p_ = nullptr;          // binary16 [max_call_tokens, p_width]
     void* a3_ = nullptr;         // binary16 [max_call_tokens, intermediate]
+    std::int8_t* a1_s8_ = nullptr;  // mlp_s8: the MLP's input and its SwiGLU in bytes, [max_call_tokens, hidden] and [.., intermediate], a scale a token
+    std::int8_t* a3_s8_ = nullptr;
+    float* a1_scales_ = nullptr;
+    float* a3_scales_ = nullptr;
     void* q_ = nullptr;          // binary16 [max_call_tokens, attn_o]: normed, rotated queries
     void* a2_ = nullptr;         // binary16 [max_call_tokens, attn_o]: the attention output, o_proj's operand
     std::size_t cache_tokens_ = 0;

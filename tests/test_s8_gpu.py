@@ -509,3 +509,119 @@ def test_refusals_of_the_library(ctx):
     assert lib.sepal_b200_rms_norm_s8(h, None, 64, None, 0, 0, None, None, None, 64, None, None, 0, 0, 64, 1e-6, None) == 0
     assert lib.sepal_b200_quantize_tokens_s8(h, None, 64, 1, None, None, 64, None, None, 0, 0, 64, None) == 0
     assert lib.sepal_b200_gemm_s8(h, None, 64, None, None, 64, None, None, 64, 0, 0, 64, 64, 0, -1, None) == 0
+
+
+def trunk_config(**kw):
+    base = dict(layers=5, hidden=256, intermediate=384, vocab=500, attn_q=256, attn_kv=64, dn_in=512, dn_v_offset=256, dn_v=128, max_call_tokens=300, mlp_int8=2, eps=1e-6, seed=11)
+    base.update(kw)
+    return sb.TrunkConfig(**base)
+
+
+def trunk_by_calls(ctx, trunk, cfg, tokens):
+    """The trunk's layer loop through the public calls, with its own weights."""
+    lib, h, inner = ctx._lib, cfg.hidden, cfg.intermediate
+    weight = lambda name, layer=0, *shape: torch.from_numpy(trunk.weight(name, layer).copy()).cuda().reshape(*shape) if shape else torch.from_numpy(trunk.weight(name, layer).copy()).cuda()  # noqa: E731
+    table, ids = weight("embedding", 0, cfg.vocab, h), torch.tensor(tokens, dtype=torch.int32, device="cuda")
+    t = len(tokens)
+    x, a = torch.empty((t, h), device="cuda"), torch.empty((t, h), dtype=torch.float16, device="cuda")
+    stream = ctx._stream(None)
+    for layer in range(cfg.layers):
+        gain = weight("norm_in", layer)
+        if layer == 0:
+            assert lib.sepal_b200_embed_rms_norm_half(table.data_ptr(), ids.data_ptr(), x.data_ptr(), gain.data_ptr(), a.data_ptr(), h, t, h, cfg.vocab, cfg.eps, stream) == 0
+        else:
+            assert lib.sepal_b200_rms_norm_half(x.data_ptr(), h, gain.data_ptr(), a.data_ptr(), h, t, h, cfg.eps, stream) == 0
+        attention = layer % 4 == 3
+        width = cfg.attn_q + 2 * cfg.attn_kv if attention else cfg.dn_in
+        mixed = ctx.gemm_f16(a, weight("mix_in", layer, width, h))
+        band = mixed[:, : cfg.attn_q] if attention else mixed[:, cfg.dn_v_offset : cfg.dn_v_offset + cfg.dn_v]
+        ctx.gemm_f16(band, weight("mix_out", layer, h, band.shape[1]), x, epilogue=sb.ADD)
+        q, s = ctx.rms_norm_s8(x, weight("norm_post", layer), eps=cfg.eps)
+        inside = ctx.gemm_s8(q, s, weight("gate_up", layer, 2 * inner, h), weight("gate_up_scales", layer), epilogue=sb.SWIGLU)
+        q, s = ctx.quantize_tokens_s8(inside)
+        ctx.gemm_s8(q, s, weight("down", layer, h, inner), weight("down_scales", layer), x, epilogue=sb.ADD)
+        torch.cuda.synchronize()
+    return x
+
+
+@pytest.mark.parametrize("n", [1, 37, 300])
+def test_a_trunk_with_its_mlp_in_eight_bits(n):
+    """mlp_int8 2 is the public calls one after the other, to the bit; its weights are the binary16 trunk's, quantised a row at a time."""
+    import numpy as np
+
+    cfg = trunk_config()
+    trunk, ctx = sb.Trunk(0, cfg), sb.Context(0)
+    tokens = np.random.default_rng(n).integers(0, cfg.vocab, n).astype(np.uint32)
+    last, hidden = trunk.run(tokens, want_all=True)[:2]
+    want = trunk_by_calls(ctx, trunk, cfg, tokens.astype(np.int64))
+    ctx.check_status()
+    assert np.array_equal(hidden, want.cpu().numpy()) and np.array_equal(last, hidden[-1])
+    half = sb.Trunk(0, trunk_config(mlp_int8=0))
+    for name, rows, k in (("gate_up", 2 * cfg.intermediate, cfg.hidden), ("down", cfg.hidden, cfg.intermediate)):
+        w = torch.from_numpy(half.weight(name, 2).copy()).cuda().reshape(rows, k)
+        q, s = ctx.quantize_rows_s8(w)
+        assert np.array_equal(trunk.weight(name, 2), q.cpu().numpy().reshape(-1)) and np.array_equal(trunk.weight(name + "_scales", 2), s.cpu().numpy())
+    ctx.close()
+
+
+def test_a_trunk_in_eight_bits_scores_requests_as_it_runs_them():
+    """Requests that share calls: the projections beside the MLP choose their schedules by the rows of a call, so the agreement is the other
+    trunks' (float32 sums in another order, amplified by the layers), and the MLP's own bits are a token's alone."""
+    import numpy as np
+
+    cfg = trunk_config(max_call_tokens=64)
+    trunk = sb.Trunk(0, cfg)
+    rng = np.random.default_rng(3)
+    requests = [rng.integers(0, cfg.vocab, n).astype(np.uint32) for n in (5, 1, 90, 33, 64)]
+    last, _ = trunk.score(requests)
+    again, _ = trunk.score(requests)
+    assert np.array_equal(last, again) and np.isfinite(last).all()
+    for r, request in enumerate(requests):
+        alone = trunk.run(request)[0]
+        # up to 4.5e-4 between the two forms (as in the binary16 trunk) is 4.5e-4 * 127 / 4 of a step of a typical byte: about 1.4 % of the bytes fall the
+        # other way, each by a step of 1 / 127 of the largest, 1 / 32 of the root mean square: sqrt(0.014) / 32 = 3.7e-3 of an MLP's input, twice a layer
+        assert np.linalg.norm(last[r] - alone) <= 1e-2 * np.linalg.norm(alone)
+
+
+def test_a_trunk_in_eight_bits_from_files(tmp_path):
+    """Saved and opened again: the same weights and results; a file of another storage is refused."""
+    import numpy as np
+
+    cfg = trunk_config()
+    trunk = sb.Trunk(0, cfg)
+    path = str(tmp_path / "placed.safetensors")
+    trunk.save(path)
+    checkpoint = sb.Checkpoint(path)
+    copy = sb.Trunk(0, cfg, checkpoint)
+    tokens = np.arange(20, dtype=np.uint32)
+    assert np.array_equal(trunk.run(tokens)[0], copy.run(tokens)[0]) and copy.weight_bytes == trunk.weight_bytes
+    for other in (0, 1):
+        with pytest.raises(sb.SepalB200Error, match="mlp_int8"):
+            sb.Trunk(0, trunk_config(mlp_int8=other), checkpoint)
+
+
+def test_a_trunk_in_eight_bits_from_a_checkpoint(tmp_path):
+    """The reference's tensor names: gate and up interleaved and quantised a row at a time from their binary16 form."""
+    import numpy as np
+
+    cfg = trunk_config(layers=1)
+    h, inner = cfg.hidden, cfg.intermediate
+    rng = np.random.default_rng(8)
+    tensor = lambda *shape: (rng.standard_normal(shape) * 0.05).astype(np.float32)  # noqa: E731
+    gate, up, down = tensor(inner, h), tensor(inner, h), tensor(h, inner)
+    pre = "layers.0."
+    tensors = {"embed_tokens.weight": tensor(cfg.vocab, h), pre + "input_layernorm.weight": tensor(h), pre + "post_attention_layernorm.weight": tensor(h),
+               pre + "linear_attn.in_proj_qkv.weight": tensor(384, h), pre + "linear_attn.in_proj_z.weight": tensor(112, h), pre + "linear_attn.in_proj_b.weight": tensor(8, h),
+               pre + "linear_attn.in_proj_a.weight": tensor(8, h), pre + "linear_attn.out_proj.weight": tensor(h, cfg.dn_v), pre + "mlp.gate_proj.weight": gate,
+               pre + "mlp.up_proj.weight": up, pre + "mlp.down_proj.weight": down}
+    path = str(tmp_path / "model.safetensors")
+    sb.write_tensor_file(path, tensors)
+    trunk, ctx = sb.Trunk(0, cfg, sb.Checkpoint(path)), sb.Context(0)
+    stacked = torch.from_numpy(np.concatenate([gate, up])).cuda().half()
+    for name, w in (("gate_up", ctx.pack_gate_up(stacked)), ("down", torch.from_numpy(down).cuda().half())):
+        q, s = ctx.quantize_rows_s8(w)
+        assert np.array_equal(trunk.weight(name), q.cpu().numpy().reshape(-1)) and np.array_equal(trunk.weight(name + "_scales"), s.cpu().numpy())
+    tokens = np.arange(9, dtype=np.uint32)
+    hidden = trunk.run(tokens, want_all=True)[1]
+    assert np.array_equal(hidden, trunk_by_calls(ctx, trunk, cfg, tokens.astype(np.int64)).cpu().numpy())
+    ctx.close()
