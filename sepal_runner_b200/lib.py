@@ -132,41 +132,35 @@ def _stream_ptr(stream) -> int:
     return int(torch.cuda.current_stream().cuda_stream) if raw is None else raw(torch.cuda.current_device())
 
 
-_TORCH = None
+# torch and what the 8-bit calls ask of it at every call, looked up once (_torch): at one token the checks of a call are what it costs.
+_TORCH = _I8 = _F16 = _F32 = _RAW_STREAM = None
 
 
 def _torch():
-    """The torch module, imported at the first call that needs it (an import statement costs each call a lookup)."""
-    global _TORCH
+    global _TORCH, _I8, _F16, _F32, _RAW_STREAM
     if _TORCH is None:
         import torch
 
+        _I8, _F16, _F32 = torch.int8, torch.float16, torch.float32
+        _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         _TORCH = torch
     return _TORCH
 
 
-def _matrix(t, dtypes, device: int):
-    """(rows, columns, row stride) of a matrix of one of `dtypes` on cuda:`device` whose rows are contiguous, or None. A lone row's stride, to
-    which torch may give any value, is said to be its length. (Few and cheap questions: at one token a call's checks are what it costs.)"""
-    if t.dtype not in dtypes or t.get_device() != device:
-        return None
-    shape = t.shape
-    if len(shape) != 2:
-        return None
-    rows, columns = shape
-    ld, step = t.stride()
-    if step != 1 and columns > 1 and rows > 0:
-        return None
-    return rows, columns, ld if rows > 1 else columns
+def _require_matrix(who: str, what: str, t, dtypes, device: int, rows=None, columns=None) -> None:
+    """Raises unless t is a [rows, columns] (None: any) matrix of one of `dtypes` on cuda:`device` whose rows are contiguous."""
+    shape = tuple(t.shape)
+    if (t.dtype in dtypes and t.get_device() == device and len(shape) == 2 and rows in (None, shape[0]) and columns in (None, shape[1]) and
+            (t.stride(1) == 1 or shape[1] <= 1 or shape[0] == 0)):
+        return
+    kinds = " or ".join(str(d).replace("torch.", "") for d in dtypes)
+    raise ValueError(f"{who}: {what} must be {kinds} [{'any' if rows is None else rows}, {'any' if columns is None else columns}] on cuda:{device} with contiguous rows, "
+                     f"not {t.dtype} {shape} of strides {t.stride()} on {t.device}")
 
 
-def _vector(t, n: int, device: int) -> bool:
-    """Whether t is n contiguous float32 values on cuda:`device`."""
-    return t.dtype is _TORCH.float32 and t.get_device() == device and t.numel() == n and t.is_contiguous()
-
-
-def _wanted(who: str, what: str, kinds: str, device: int, t) -> str:
-    return f"{who}: {what} must be {kinds} on cuda:{device} with contiguous rows, not {t.dtype} {tuple(t.shape)} of stride {t.stride()} on {t.device}"
+def _require_vector(who: str, what: str, t, n: int, device: int) -> None:
+    if t.dtype is not _F32 or t.get_device() != device or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{who}: {what} must be {n} contiguous float32 values on cuda:{device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 @dataclass
@@ -334,107 +328,136 @@ class Context:
         return y
 
     # ---- activations in 8 bits ---------------------------------------------------------------------------------------------
+    # Each call asks what the C ABI cannot see in one expression; only a call that fails it is taken apart for the message. A lone row's stride,
+    # to which torch may give any value, is never used: the row's length goes in its place.
     def _stream(self, stream) -> int:
         """The cudaStream_t of `stream`, or of the current stream of the context's device (which need not be the current one)."""
         if stream is not None:
             return int(stream.cuda_stream)
-        raw = getattr(_TORCH._C, "_cuda_getCurrentRawStream", None)
-        return int(_TORCH.cuda.current_stream(self.device).cuda_stream) if raw is None else raw(self.device)
+        return _RAW_STREAM(self.device) if _RAW_STREAM is not None else int(_torch().cuda.current_stream(self.device).cuda_stream)
 
-    def _row_operands(self, who: str, t: int, c: int, q, scales, col_scale, values):
-        """What the two calls that leave int8 rows have in common: q and scales (new ones, q in rows of a multiple of 16 bytes as gemm_s8 takes
-        them, or the caller's after checks), and the pointers and strides of q, scales, col_scale and values."""
-        torch, device = _TORCH, self.device
+    def _rows_call(self, call, who: str, head, t: int, c: int, q, scales, col_scale, values, tail, stream):
+        """What the two calls that leave int8 rows have in common: q and scales (new ones, q in rows of a multiple of 16 bytes as gemm_s8
+        takes them, or the caller's), col_scale and values checked, and the call."""
+        device = self.device
         if q is None:
             ld_q = (c + 15) // 16 * 16
-            q = torch.empty((t, ld_q), dtype=torch.int8, device=f"cuda:{device}")[:, :c]
+            q = _TORCH.empty((t, ld_q), dtype=_I8, device=f"cuda:{device}")[:, :c]
         else:
-            got = _matrix(q, (torch.int8,), device)
-            if got is None or got[0] != t or got[1] != c:
-                raise ValueError(_wanted(who, "q", f"int8 [{t}, {c}]", device, q))
-            ld_q = got[2]
+            if q.dtype is not _I8 or q.get_device() != device or q.shape != (t, c):
+                _require_matrix(who, "q", q, (_I8,), device, t, c)
+            ld_q, step = q.stride()
+            if step != 1:
+                _require_matrix(who, "q", q, (_I8,), device, t, c)
+            if t < 2:
+                ld_q = c
         if scales is None:
-            scales = torch.empty((t,), dtype=torch.float32, device=f"cuda:{device}")
-        elif not _vector(scales, t, device):
-            raise ValueError(_wanted(who, "scales", f"{t} float32 values", device, scales))
-        smooth = stands = None
-        ld_stands = 0
+            scales = _TORCH.empty((t,), dtype=_F32, device=f"cuda:{device}")
+        elif scales.dtype is not _F32 or scales.get_device() != device or scales.numel() != t or not scales.is_contiguous():
+            _require_vector(who, "scales", scales, t, device)
+        smooth, stands, ld_stands = None, None, 0
         if col_scale is not None:
-            if not _vector(col_scale, c, device):
-                raise ValueError(_wanted(who, "col_scale", f"{c} float32 values", device, col_scale))
+            _require_vector(who, "col_scale", col_scale, c, device)
             smooth = col_scale.data_ptr()
         if values is not None:
-            got = _matrix(values, (torch.float16,), device)
-            if got is None or got[0] != t or got[1] != c:
-                raise ValueError(_wanted(who, "values", f"float16 [{t}, {c}]", device, values))
-            stands, ld_stands = values.data_ptr(), got[2]
-        return q, scales, (smooth, q.data_ptr(), ld_q, scales.data_ptr(), stands, ld_stands)
+            if values.dtype is not _F16 or values.get_device() != device or values.shape != (t, c):
+                _require_matrix(who, "values", values, (_F16,), device, t, c)
+            ld_stands, step = values.stride()
+            if step != 1:
+                _require_matrix(who, "values", values, (_F16,), device, t, c)
+            if t < 2:
+                ld_stands = c
+            stands = values.data_ptr()
+        if call(self._h, *head, smooth, q.data_ptr(), ld_q, scales.data_ptr(), stands, ld_stands, t, c, *tail, self._stream(stream)) != 0:
+            _check(1)
+        return q, scales
 
     def rms_norm_s8(self, x, w, q=None, scales=None, *, delta=None, col_scale=None, eps: float = 1e-6, values=None, stream=None):
         """The residual's addition (x += delta, in place; delta None: x is only read), the zero-centred RMSNorm and one int8 row with a
         float32 scale a token (sepal_b200_rms_norm_s8). x float32 [T, C], w float32 [C], delta float16 or float32 [T, C], col_scale float32
         [C] (smoothing factors), values None or float16 [T, C], which gets what the bytes stand for; returns (q int8 [T, C], scales float32
         [T])."""
-        torch, device = _torch(), self.device
-        got = _matrix(x, (torch.float32,), device)
-        if got is None:
-            raise ValueError(_wanted("rms_norm_s8", "x", "float32 [T, C]", device, x))
-        t, c, ld_x = got
-        if not _vector(w, c, device):
-            raise ValueError(_wanted("rms_norm_s8", "w", f"{c} float32 values", device, w))
+        if _TORCH is None:
+            _torch()
+        device, shape = self.device, x.shape
+        if x.dtype is not _F32 or x.get_device() != device or len(shape) != 2:
+            _require_matrix("rms_norm_s8", "x", x, (_F32,), device)
+        t, c = shape
+        ld_x, step = x.stride()
+        if step != 1:
+            _require_matrix("rms_norm_s8", "x", x, (_F32,), device)
+        if t < 2:
+            ld_x = c
+        if w.dtype is not _F32 or w.get_device() != device or w.numel() != c or not w.is_contiguous():
+            _require_vector("rms_norm_s8", "w", w, c, device)
         added, ld_added, half = None, 0, 0
         if delta is not None:
-            got = _matrix(delta, (torch.float16, torch.float32), device)
-            if got is None or got[0] != t or got[1] != c:
-                raise ValueError(_wanted("rms_norm_s8", "delta", f"float16 or float32 [{t}, {c}]", device, delta))
-            added, ld_added, half = delta.data_ptr(), got[2], 1 if delta.dtype is torch.float16 else 0
-        q, scales, rest = self._row_operands("rms_norm_s8", t, c, q, scales, col_scale, values)
-        _check(self._lib.sepal_b200_rms_norm_s8(self._h, x.data_ptr(), ld_x, added, ld_added, half, w.data_ptr(), *rest, t, c, eps, self._stream(stream)))
-        return q, scales
+            _require_matrix("rms_norm_s8", "delta", delta, (_F16, _F32), device, t, c)
+            added, ld_added, half = delta.data_ptr(), delta.stride(0) if t > 1 else c, 1 if delta.dtype is _F16 else 0
+        return self._rows_call(self._lib.sepal_b200_rms_norm_s8, "rms_norm_s8", (x.data_ptr(), ld_x, added, ld_added, half, w.data_ptr()), t, c, q, scales, col_scale,
+                               values, (eps,), stream)
 
     def quantize_tokens_s8(self, x, q=None, scales=None, *, col_scale=None, values=None, stream=None):
         """One int8 row with a float32 scale a token (sepal_b200_quantize_tokens_s8): x float16 or float32 [T, K] (times col_scale, float32
         [K]), values None or float16 [T, K], which gets what the bytes stand for; returns (q int8 [T, K], scales float32 [T])."""
-        torch, device = _torch(), self.device
-        got = _matrix(x, (torch.float16, torch.float32), device)
-        if got is None:
-            raise ValueError(_wanted("quantize_tokens_s8", "x", "float16 or float32 [T, K]", device, x))
-        t, k, ld_x = got
-        q, scales, rest = self._row_operands("quantize_tokens_s8", t, k, q, scales, col_scale, values)
-        _check(self._lib.sepal_b200_quantize_tokens_s8(self._h, x.data_ptr(), ld_x, 1 if x.dtype is torch.float16 else 0, *rest, t, k, self._stream(stream)))
-        return q, scales
+        if _TORCH is None:
+            _torch()
+        device, shape, kind = self.device, x.shape, x.dtype
+        if (kind is not _F16 and kind is not _F32) or x.get_device() != device or len(shape) != 2:
+            _require_matrix("quantize_tokens_s8", "x", x, (_F16, _F32), device)
+        t, k = shape
+        ld_x, step = x.stride()
+        if step != 1:
+            _require_matrix("quantize_tokens_s8", "x", x, (_F16, _F32), device)
+        if t < 2:
+            ld_x = k
+        return self._rows_call(self._lib.sepal_b200_quantize_tokens_s8, "quantize_tokens_s8", (x.data_ptr(), ld_x, 1 if kind is _F16 else 0), t, k, q, scales, col_scale,
+                               values, (), stream)
 
     def gemm_s8(self, xq, sx, wq, sw, y=None, *, epilogue: int = STORE, y_half: bool = True, config: int = -1, stream=None):
         """y = epilogue(float(xq @ wq.T) * sx[:, None] * sw): xq int8 [T, K] with sx float32 [T] (rms_norm_s8, quantize_tokens_s8), wq int8
         [N, K] with sw float32 [N] (quantize_rows_s8). The sums are exact integers (sepal_b200_gemm_s8)."""
-        torch, device = _torch(), self.device
-        got, weights = _matrix(xq, (torch.int8,), device), _matrix(wq, (torch.int8,), device)
-        if got is None:
-            raise ValueError(_wanted("gemm_s8", "xq", "int8 [T, K]", device, xq))
-        if weights is None:
-            raise ValueError(_wanted("gemm_s8", "wq", "int8 [N, K]", device, wq))
-        t, k, ld_x = got
-        n, wk, ld_w = weights
-        if wk != k:
-            raise ValueError(f"gemm_s8: xq is [{t}, {k}] but wq is [{n}, {wk}]: the inner dimensions must agree")
-        if not _vector(sx, t, device):
-            raise ValueError(_wanted("gemm_s8", "sx", f"{t} float32 values", device, sx))
-        if not _vector(sw, n, device):
-            raise ValueError(_wanted("gemm_s8", "sw", f"{n} float32 values", device, sw))
+        if _TORCH is None:
+            _torch()
+        device, x_shape, w_shape = self.device, xq.shape, wq.shape
+        if xq.dtype is not _I8 or xq.get_device() != device or len(x_shape) != 2:
+            _require_matrix("gemm_s8", "xq", xq, (_I8,), device)
+        t, k = x_shape
+        if wq.dtype is not _I8 or wq.get_device() != device or len(w_shape) != 2 or w_shape[1] != k:
+            _require_matrix("gemm_s8", "xq", xq, (_I8,), device)
+            _require_matrix("gemm_s8", "wq", wq, (_I8,), device)
+            raise ValueError(f"gemm_s8: xq is [{t}, {k}] but wq is {tuple(w_shape)}: the inner dimensions must agree")
+        n = w_shape[0]
+        (ld_x, x_step), (ld_w, w_step) = xq.stride(), wq.stride()
+        if x_step != 1 or w_step != 1:
+            _require_matrix("gemm_s8", "xq", xq, (_I8,), device)
+            _require_matrix("gemm_s8", "wq", wq, (_I8,), device)
+        if t < 2:
+            ld_x = (k + 15) // 16 * 16
+        if n < 2:
+            ld_w = (k + 15) // 16 * 16
+        if (sx.dtype is not _F32 or sx.get_device() != device or sx.numel() != t or not sx.is_contiguous() or
+                sw.dtype is not _F32 or sw.get_device() != device or sw.numel() != n or not sw.is_contiguous()):
+            _require_vector("gemm_s8", "sx", sx, t, device)
+            _require_vector("gemm_s8", "sw", sw, n, device)
         columns = n // 2 if epilogue == SWIGLU else n
         if y is None:
             if epilogue == ADD:
                 raise ValueError("gemm_s8: epilogue ADD updates an output that the caller gives")
-            y, ld_y = torch.empty((t, columns), dtype=torch.float16 if y_half else torch.float32, device=xq.device), columns
+            y, ld_y = _TORCH.empty((t, columns), dtype=_F16 if y_half else _F32, device=xq.device), columns
         else:
-            got = _matrix(y, (torch.float16, torch.float32), device)
-            if got is None or got[0] != t or got[1] != columns:
-                raise ValueError(_wanted("gemm_s8", "the output", f"float16 or float32 [{t}, {columns}]", device, y))
-            y_half, ld_y = y.dtype is torch.float16, got[2]
-        # (a lone row's stride is never used: one that the kernels take)
-        _check(self._lib.sepal_b200_gemm_s8(self._h, xq.data_ptr(), ld_x if t > 1 else (k + 15) // 16 * 16, sx.data_ptr(), wq.data_ptr(),
-                                            ld_w if n > 1 else (k + 15) // 16 * 16, sw.data_ptr(), y.data_ptr(), ld_y, 1 if y_half else 0, t, n, k, epilogue,
-                                            config, self._stream(stream)))
+            kind = y.dtype
+            y_half = kind is _F16
+            if (not y_half and kind is not _F32) or y.get_device() != device or y.shape != (t, columns):
+                _require_matrix("gemm_s8", "the output", y, (_F16, _F32), device, t, columns)
+            ld_y, step = y.stride()
+            if step != 1:
+                _require_matrix("gemm_s8", "the output", y, (_F16, _F32), device, t, columns)
+            if t < 2:
+                ld_y = columns
+        if self._lib.sepal_b200_gemm_s8(self._h, xq.data_ptr(), ld_x, sx.data_ptr(), wq.data_ptr(), ld_w, sw.data_ptr(), y.data_ptr(), ld_y, 1 if y_half else 0,
+                                        t, n, k, epilogue, config, self._stream(stream)) != 0:
+            _check(1)
         return y
 
     def pack_gate_up(self, stacked, stream=None):
