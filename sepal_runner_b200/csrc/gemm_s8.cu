@@ -751,6 +751,8 @@ void launch_gemm_s8(Context& ctx, const std::int8_t* x, std::size_t ld_x, const 
     if (x == nullptr || w == nullptr || sx == nullptr || sw == nullptr || y == nullptr) throw std::invalid_argument("launch_gemm_s8: null pointer");
     if (reinterpret_cast<std::uintptr_t>(x) % 16 != 0 || reinterpret_cast<std::uintptr_t>(w) % 16 != 0)
         throw std::invalid_argument("launch_gemm_s8: X and W must be 16-byte aligned");
+    if (reinterpret_cast<std::uintptr_t>(sx) % 4 != 0 || reinterpret_cast<std::uintptr_t>(sw) % 4 != 0 || reinterpret_cast<std::uintptr_t>(y) % (y_half ? 2 : 4) != 0)
+        throw std::invalid_argument("launch_gemm_s8: a pointer is not aligned to its values");
     const std::size_t pair_tiles_at_most = (t + 31) / 32 * ((n + 255) / 256);
     if (pair_tiles_at_most > 0x7FFFFFFFu) throw std::invalid_argument("launch_gemm_s8: too many output tiles for one call");
     check(cudaSetDevice(ctx.device), "cudaSetDevice");

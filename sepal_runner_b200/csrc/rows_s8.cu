@@ -383,6 +383,8 @@ void launch_rms_norm_s8(const Context& ctx, float* x, std::size_t ld_x, const vo
     if (!(eps >= 1.0e-30f) || !std::isfinite(eps)) throw std::invalid_argument("launch_rms_norm_s8: eps must be a positive number (1e-30 at least)");
     if (rows == 0) return;
     if (x == nullptr || w == nullptr || q == nullptr || scales == nullptr) throw std::invalid_argument("launch_rms_norm_s8: null pointer");
+    if (!aligned(x, 4) || !aligned(w, 4) || !aligned(scales, 4) || !aligned(col_scale, 4) || !aligned(delta, delta_half ? 2 : 4) || !aligned(values, 2))
+        throw std::invalid_argument("launch_rms_norm_s8: a pointer is not aligned to its values");
     check(cudaSetDevice(ctx.device), "cudaSetDevice");
     const RowsParams p{x, ld_x, delta, ld_delta, w, col_scale, q, ld_q, scales, static_cast<__half*>(values), ld_values, cols, eps};
     const unsigned kind = delta == nullptr ? 0u : delta_half ? 1u : 2u;
@@ -405,6 +407,8 @@ void launch_quantize_tokens_s8(const Context& ctx, const void* x, std::size_t ld
     check_rows("launch_quantize_tokens_s8", rows, cols, ld_x, ld_q, values, ld_values);
     if (rows == 0) return;
     if (x == nullptr || q == nullptr || scales == nullptr) throw std::invalid_argument("launch_quantize_tokens_s8: null pointer");
+    if (!aligned(x, x_half ? 2 : 4) || !aligned(scales, 4) || !aligned(col_scale, 4) || !aligned(values, 2))
+        throw std::invalid_argument("launch_quantize_tokens_s8: a pointer is not aligned to its values");
     check(cudaSetDevice(ctx.device), "cudaSetDevice");
     const RowsParams p{x, ld_x, nullptr, 0, nullptr, col_scale, q, ld_q, scales, static_cast<__half*>(values), ld_values, cols, 0.0f};
     const std::size_t per_vec = x_half ? 8 : 4;
