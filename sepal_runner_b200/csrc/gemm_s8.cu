@@ -8,9 +8,21 @@
 // nothing is computed for tokens that are not there.
 //
 //   gemm_s8_pair_kernel  CTA pairs, 256 weight rows by `bt` tokens to a tile, persistent, two accumulators in tensor memory (the epilogue of a
-//                        tile runs behind the next tile's products). From a few hundred tokens up.
-//   gemm_s8_few_kernel   up to 256 tokens, where reading the weights once is what the call costs: 128 weight rows to a CTA, a tile's k cut
-//                        over a cluster of up to eight CTAs, whose sums meet through distributed shared memory.
+//                        tile runs behind the next tile's products).
+//   gemm_s8_few_kernel   up to 256 tokens, where a few weight rows have a long k: 128 weight rows to a CTA, a tile's k cut over a cluster of up to
+//                        eight CTAs, whose sums meet through distributed shared memory.
+//
+// What bounds them, and what they measured (launches back to back, weights from DRAM, clocks as they were):
+//   - Full calls are bound by the tensor cores under the power cap: 4096 x 24576 x 4096 with SwiGLU 251 us in bursts (3.28 POP/s, where the
+//     measured binary16 rate of the library product, doubled, is 3.31) and 270 to 280 over a quarter of a second.
+//   - A few hundred tokens make one to five waves of tiles; a step takes the 2 bt clocks of its MMAs (310 to 316 measured at bt 160), and what
+//     is lost is the part of the last wave without tiles and about 10,000 clocks a launch: 3000 until the launch before has ended, 1100 for
+//     the first boxes, 4100 for the last tile's results (all pairs add theirs at once; leaving them lane by lane without the staging
+//     boxes takes as long, and longer in binary16) and 1400 to leave. 900 x 2560 x 9728 added: 20.3 us (2.2 POP/s); 1337 x 6144 x 2560
+//     16.9; 900 x 19456 x 2560 SwiGLU 36.
+//   - Few tokens are bound by the launch (3.3 us with next to nothing to do) and then the reading of W: one token by 6144 x 2560 5.6 us, 2560 x 9728
+//     7.4, 24576 x 4096 18.5 (15.4 at the memory's rate).
+//   Requesting W ahead into the L2 changed nothing; nor did fewer commits.
 #include "gemm_s8.hpp"
 
 #include <atomic>
@@ -58,7 +70,7 @@ __device__ __forceinline__ float scaled(int sum, float sx, float sw) { return __
 //   warp 1      MMA issuer (first CTA): four tcgen05.mma.cta_group::2 (M 256, N bt, K 32) to a step
 //   warps 2..9  epilogue: two warps to a quarter of the accumulator's lanes, which take chunks of 32 tokens in turn. A lane is an output
 //               column, its registers run along the tokens; a chunk leaves transposed through the warp's staging boxes and the TMA (a store,
-//               or a reduce-add for the float32 residual update), or lane by lane where Y's rows are not 16-byte aligned.
+//               or a reduce-add for the float32 residual update), or lane by lane where Y's rows are not whole 16-byte units.
 constexpr unsigned kPairThreads = 320;
 constexpr unsigned kMaxStages = 12;
 constexpr unsigned kAccStride = 256;          // tensor-memory columns from one accumulator to the other
@@ -420,6 +432,9 @@ gemm_s8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 //   warp 1      MMA issuer (M 128, N up to 256, K 32); a slot is committed back only where it is loaded again
 //   warps 2..9  epilogue: the sums into shared memory, [token][row of W]; behind the cluster's barrier the parts of a token are added by the
 //               CTA whose token it is (token mod split) and leave in rows of 128 consecutive columns.
+//
+// 2560 weight rows by k 9728 are ten tiles for 74 pairs: one token takes 12.3 us there and 7.4 here, cut in eight. The exchange costs 0.03 us a
+// token (64 tokens 9.8 us, 128 tokens 11.5), so that the two are level at about 200 tokens, and at 16 to 64 with a shorter k or more rows.
 constexpr unsigned kFewThreads = 320;
 constexpr unsigned kFewBarriers = 2 * kMaxStages + 1;
 constexpr unsigned kFewTail = kFewBarriers * 8 + 64;
