@@ -295,12 +295,13 @@ gemm_s8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         for (unsigned tile = pair; tile < p.tiles; tile += pairs) {
             const unsigned row0 = tile / p.t_tiles * 256 + rank * kRows, t0 = tile % p.t_tiles * bt;
             const unsigned n = row0 + quarter * 32 + lane;
-            const float sw = n < p.n ? __ldg(p.sw + n) : 0.0f;
+            // (plain loads: the kernel before this one, which may have left the scales, can still run when this one starts)
+            const float sw = n < p.n ? p.sw[n] : 0.0f;
             float sx[4];
 #pragma unroll
             for (unsigned i = 0; i < 4; ++i) {
                 const unsigned token = t0 + 64 * i + 32 * turn + lane;
-                sx[i] = 64 * i + 32 * turn < bt && token < p.m ? __ldg(p.sx + token) : 0.0f;
+                sx[i] = 64 * i + 32 * turn < bt && token < p.m ? p.sx[token] : 0.0f;
             }
             bool go = wait_barrier(acc_full_bar(acc), acc_phase, abort_flag, p.status, kStatusEpilogueAccFull);
             go = __all_sync(0xFFFFFFFFu, go) && *abort_flag == 0;
@@ -610,10 +611,10 @@ gemm_s8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 #pragma unroll
         for (unsigned i = 0; i < 4; ++i) {
             const unsigned n = row0 + (gated ? at + i % 2 + (i / 2) * 64 : at + i);
-            sw[i] = n < p.n ? __ldg(p.sw + n) : 0.0f;
+            sw[i] = n < p.n ? p.sw[n] : 0.0f;
         }
         for (unsigned token = rank + p.split * worker; token < p.m; token += kEpilogueWarps * p.split) {
-            const float sx = __ldg(p.sx + token);
+            const float sx = p.sx[token];
             const uint32_t here = base + token * (kRows * 4) + at * 4;
             int4 part[8];
 #pragma unroll

@@ -259,6 +259,7 @@ def check_multiply(ctx, t, n, k, configs, seed=3):
     gen, x, sx, w, sw = operands(seed, t, n, k)
     want = product(x, w, sx, sw)
     old = randn(gen, t, n)
+    gated = None
     for config in configs:
         for aligned in (True, False):
             for dtype in (torch.float32, torch.float16):
@@ -279,6 +280,8 @@ def check_multiply(ctx, t, n, k, configs, seed=3):
                         slack = slack + value.abs() * 2.0**-11 + 2.0**-25
                     assert ((y.double() - value).abs() <= slack).all(), (config, aligned, dtype)
                     untouched()
+                    gated = y.clone() if gated is None else gated
+                    assert torch.equal(y, gated.to(dtype))  # (the first is float32) the same bits whatever the schedule
     ctx.check_status()
 
 
@@ -459,6 +462,34 @@ def test_a_captured_mlp_replays_on_new_inputs(ctx):
     own.check_status()
     del graph
     own.close()
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 512, 1024), (40, 512, 2048), (300, 1024, 512)])
+def test_buffers_used_again_without_a_wait(t, n, k):
+    """Norm, product, norm, product on one stream into the same bytes and scales, each launched while the one before still runs: every product
+    is of its own norm's rows, and none of those is overwritten early."""
+    c = sb.Context(0)
+    c.set_static_weights(True)
+    gen = generator(t)
+    w = randn(gen, k, std=0.3)
+    wq, sw = c.quantize_rows_s8(randn(gen, n, k, std=0.05).half())
+    xs = [randn(gen, t, k, std=1.0 + i) for i in range(40)]
+    want = []
+    for x in xs:
+        q, s = c.rms_norm_s8(x, w)
+        want.append(product(q, wq, s, sw))
+    q, s = torch.empty((t, k), dtype=torch.int8, device="cuda"), torch.empty(t, device="cuda")
+    got = [torch.empty((t, n), device="cuda") for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for x, y in zip(xs, got):
+            c.rms_norm_s8(x, w, q, s)
+            c.gemm_s8(q, s, wq, sw, y)
+        c.check_status()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for y in got:
+            y.zero_()
+    c.close()
 
 
 def test_two_streams_with_a_context_each():
