@@ -8,7 +8,8 @@
 // reduction and the rounding, a thread up to four vectors of 16 bytes (a 2560-wide float32 row is 160 threads, a 9728-wide binary16 row
 // 320), all of whose loads are issued before the first is used and leave the L1 to the gains. With two vectors to a thread a single row
 // is 0.3 us faster and 4096 rows of 4096 values 3.6 us slower (23.1 and 19.5); a ring of rows in shared memory, filled by bulk copies
-// while groups of warps round, was built and was 10 to 30 % slower but for 48 KB rows without gains. Rows wider than 768 threads hold are
+// while groups of warps round, was built and was 10 to 30 % slower but for 48 KB rows without gains, and persistent blocks that load their
+// next row while they reduce one were level at best. Rows wider than 768 threads hold are
 // read again behind the barrier (from the L2). Rows that are not aligned to the vectors, or whose length is odd, take a kernel of single-value
 // accesses. Measured alone, back to back, against the memory's 6.56 TB/s: 4096 x 2560, float32 delta 24.1 us (86 %), binary16 delta 20.5 (86 %);
 // 4096 x 4096 without 19.5 (66 %); quantise 4096 x 9728 binary16 22.9 (80 %), 4096 x 12288 float32 46.1 (83 %); 900 x 2560, binary16 delta 7.0
