@@ -13,6 +13,8 @@
  *     downloaded inside the call.
  *
  * Matrices are row-major; a matrix argument is a pointer and a row stride in elements (runner/cuda/src/device.hpp:14-16).
+ * Nothing outside the columns of a result's rows is written: a result may be a band of a wider matrix. (Where a text below speaks of
+ * 16-byte aligned rows of a result it means its pointer and stride; rows that are also whole 16-byte units long are the fast form.)
  *   Y[t, n] = epilogue( sum over k of X[t, k] * W[n, k] ),   X [T, K], W [N, K] (one output feature per row, K contiguous).
  *
  * There is no CPU path and no library GEMM behind these functions: on a device that is not sm_100 sepal_b200_open fails.
@@ -106,7 +108,7 @@ SEPAL_B200_API int32_t sepal_b200_set_static_weights(sepal_b200_ctx* ctx, int32_
  * SWIGLU needs N a multiple of 128. config: -1 picks the tile width and schedule from the shape; other values force one (tests and
  * tuning: 0..3, or a tile width that is a multiple of 16 up to 256, plus 1 for the even split of k, 2 for CTA pairs, 3 for both,
  * 6 for pairs that run whole tiles first and split only the last waves, and, for a float32 residual update (ADD, y_half == 0, 16-byte
- * aligned rows) only, 7 for pairs that share every tile when there are fewer tiles than pairs, or 5 for pairs that share the tiles
+ * aligned rows, N a multiple of 4) only, 7 for pairs that share every tile when there are fewer tiles than pairs, or 5 for pairs that share the tiles
  * of the last, partial wave: the parts of a shared tile are added to Y one after the other in the order of their ranges of k, two
  * or three float32 additions in a fixed order instead of one; -1 takes these forms where they are the faster ones); or 512 + w (w =
  * 64, 96, ..., 192, 256 or 320) for the kernel that takes the weights as the tensor cores' first operand with w tokens to a tile,
@@ -142,7 +144,7 @@ SEPAL_B200_API int32_t sepal_b200_gemm_f16_noalloc(const void* x, uint64_t ld_x,
  * Requires K a multiple of 128, ld_x a multiple of 8, ld_q a multiple of 16, scales_t 16-byte aligned with ld_st >= N rounded up to
  * 256 (the padding zero). config as sepal_b200_gemm_f16, and 512 + w (w = 64, 96, ..., 192, 256 or 320) forces the kernel that takes the
  * weights as the tensor cores' first operand with w tokens to a tile, which -1 picks where it is the faster one; 512 + w + 1 (a
- * float32 result, stored or added, in 16-byte aligned rows; a last wave of fewer tiles than CTA pairs) forces its shared form, in which
+ * float32 result, stored or added, in 16-byte aligned rows, N a multiple of 4; a last wave of fewer tiles than CTA pairs) forces its shared form, in which
  * the CTA pairs that would idle in that wave take the first scale groups of each of its tiles: Y becomes (Y + the first groups' product) + the other groups' product
  * (without the Y for a stored result), float32 additions in a fixed order (-1 takes this form where it is the faster one). */
 SEPAL_B200_API int32_t sepal_b200_gemm_w8g(sepal_b200_ctx* ctx, const void* x, uint64_t ld_x, const int8_t* q, uint64_t ld_q, const void* scales_t,
@@ -153,7 +155,7 @@ SEPAL_B200_API int32_t sepal_b200_gemm_w8g(sepal_b200_ctx* ctx, const void* x, u
  * the tokens to a tile of the swapped kernel (96, 128, 160 or 192: one block; 256 or 320: two blocks of half as many that share the
  * converted weights; sepal_b200_gemm_w8g's config 512 + w forces it), or 0 for the others (the unswapped kernels; the few-rows kernel,
  * up to 128 rows and up to 256 where it cuts k in four parts or more). `epilogue` as in the multiply;
- * `staged` != 0: the result goes into 16-byte aligned rows and is neither a float32 SwiGLU nor a binary16 residual update (it then
+ * `staged` != 0: the result goes into 16-byte aligned rows of whole 16-byte units (N a multiple of 4 in float32, of 8 in binary16) and is neither a float32 SwiGLU nor a binary16 residual update (it then
  * leaves through shared memory and the TMA, which the estimate counts). Host arithmetic only: needs no GPU and no context. No counterpart in the reference. */
 SEPAL_B200_API int32_t sepal_b200_w8g_schedule(uint32_t sm_count, uint64_t t, uint64_t n, uint64_t k, int32_t epilogue, int32_t staged);
 

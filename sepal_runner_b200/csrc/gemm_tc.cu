@@ -2369,6 +2369,15 @@ unsigned pick_pair_stream_k(unsigned pairs, unsigned pair_tiles, unsigned m, uns
     return w8 || idle >= 0.45 ? 1u : 0u;
 }
 
+// Whether rows of Y can leave through the TMA: 16-byte aligned, and a whole number of 16-byte units long. The TMA drops what lies past the
+// matrix in such units only (a box over the end of rows of 1010 binary16 values changes columns 1010 .. 1015 too, measured for stores and
+// reduce-adds): rows of another length, bands of a wider matrix, would have the columns behind them overwritten.
+bool tma_takes_rows(const void* y, std::size_t ld_y, std::size_t columns, bool y_half) {
+    const std::size_t unit = y_half ? 8 : 4;
+    return reinterpret_cast<std::uintptr_t>(y) % 16 == 0 && ld_y % unit == 0 && columns % unit == 0;
+}
+bool tma_takes_rows(const GemmParams& p) { return tma_takes_rows(p.y, p.ld_y, p.epilogue == 2 ? p.n / 2 : p.n, p.y_half != 0); }
+
 // The order of the tiles of a pair launch. The pairs of a wave work on consecutive tiles at about the same k, so what consecutive
 // tiles share is read from memory once per wave and what they do not share once per tile: the larger operand should be the shared
 // one. With more rows of X than of W (the down, o and DeltaNet out projections from a few thousand tokens up) consecutive tiles walk
@@ -2496,14 +2505,14 @@ void launch_w8t_pair(const Context& ctx, const void* x, std::size_t ld_x, const 
     p.k_iters = p.k / kW8Group;
     p.stream_k = 0;
     p.split_base = 0;
-    p.staged_add = (p.epilogue != 2 && p.y_half == 0 && p.vec_ok != 0) ? 1u : 0u;  // float32 results (added or stored) leave in boxes of [32 x 32]
+    p.staged_add = (p.epilogue != 2 && p.y_half == 0 && tma_takes_rows(p)) ? 1u : 0u;  // float32 results (added or stored) leave in boxes of [32 x 32]
     const CUtensorMap map_x = make_tensor_map_2d(ctx, x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.m, p.k, ld_x, bt / 2, kBK, true);
     const CUtensorMap map_w = make_tensor_map_2d(ctx, q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.n, p.k, ld_q, 128, kW8Group, true);
     CUtensorMap map_y;
     std::memset(&map_y, 0, sizeof map_y);
     if (p.staged_add != 0) map_y = make_tensor_map_2d(ctx, p.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.m, p.n, p.ld_y, 32, 32, true);
     // binary16 results that are not added to what Y holds leave through shared memory too, in boxes of 16 tokens x 32 columns
-    p.staged_store = (p.epilogue != 1 && p.y_half != 0 && reinterpret_cast<std::uintptr_t>(p.y) % 16 == 0 && (p.ld_y * 2) % 16 == 0) ? 1u : 0u;
+    p.staged_store = (p.epilogue != 1 && p.y_half != 0 && tma_takes_rows(p)) ? 1u : 0u;
     if (p.staged_store != 0)
         map_y = make_tensor_map_2d(ctx, p.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.m, p.epilogue == 2 ? p.n / 2 : p.n, p.ld_y, 16, 32, false);
     const unsigned smem = fixed + depth * per_group;
@@ -2520,7 +2529,7 @@ void launch_w8t_pair(const Context& ctx, const void* x, std::size_t ld_x, const 
     }
     if (share > 0 && given == 0)
         throw std::invalid_argument("launch_gemm_w8g: the shared form (config 512 + w + 1) needs a float32 result (stored or added) in 16-byte aligned "
-                                    "rows, a last wave of fewer tiles than CTA pairs and at least four scale groups");
+                                    "rows of whole 16-byte units, a last wave of fewer tiles than CTA pairs and at least four scale groups");
     if (given != 0) {
         p.stream_k = 1;
         p.split_base = given;
@@ -2569,13 +2578,13 @@ void launch_f16t_pair(const Context& ctx, const void* x, std::size_t ld_x, const
     p.col_scale = nullptr;
     p.scales_t = nullptr;
     p.ld_st = 0;
-    p.staged_add = (p.epilogue != 2 && p.y_half == 0 && p.vec_ok != 0) ? 1u : 0u;
+    p.staged_add = (p.epilogue != 2 && p.y_half == 0 && tma_takes_rows(p)) ? 1u : 0u;
     const CUtensorMap map_x = make_tensor_map_2d(ctx, x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.m, p.k, ld_x, bt / 2, kBK, true);
     const CUtensorMap map_w = make_tensor_map_2d(ctx, w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.n, p.k, ld_w, 128, kBK, true);
     CUtensorMap map_y;
     std::memset(&map_y, 0, sizeof map_y);
     if (p.staged_add != 0) map_y = make_tensor_map_2d(ctx, p.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.m, p.n, p.ld_y, 32, 32, true);
-    p.staged_store = (p.epilogue != 1 && p.y_half != 0 && reinterpret_cast<std::uintptr_t>(p.y) % 16 == 0 && (p.ld_y * 2) % 16 == 0) ? 1u : 0u;
+    p.staged_store = (p.epilogue != 1 && p.y_half != 0 && tma_takes_rows(p)) ? 1u : 0u;
     if (p.staged_store != 0)
         map_y = make_tensor_map_2d(ctx, p.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.m, p.epilogue == 2 ? p.n / 2 : p.n, p.ld_y, 16, 32, false);
     const unsigned smem = fixed + depth * per_step;
@@ -2656,7 +2665,7 @@ void launch_pair(const Context& ctx, const CUtensorMap& map_x, const CUtensorMap
             return;
         }
         if (stream_k == 5)
-            throw std::invalid_argument("launch_gemm_f16: config width + 5 needs a float32 residual update into 16-byte aligned rows and a last wave of tiles "
+            throw std::invalid_argument("launch_gemm_f16: config width + 5 needs a float32 residual update into 16-byte aligned rows of whole 16-byte units and a last wave of tiles "
                                         "that leaves at least half of the CTA pairs idle");
         stream_k = -1;
     }
@@ -2666,7 +2675,7 @@ void launch_pair(const Context& ctx, const CUtensorMap& map_x, const CUtensorMap
             given = pair_given(static_cast<unsigned>(max_pairs[slot]), pair_tiles, p.k_iters);
         if (given == 0 && stream_k == 4) stream_k = -1;
         if (given == 0 && stream_k == 3)
-            throw std::invalid_argument("launch_gemm_f16: the shared form (config width + 7) needs a float32 residual update into 16-byte aligned rows, "
+            throw std::invalid_argument("launch_gemm_f16: the shared form (config width + 7) needs a float32 residual update into 16-byte aligned rows of whole 16-byte units, "
                                         "fewer tiles than CTA pairs and at least eight k iterations");
     }
     unsigned pairs;
@@ -2817,7 +2826,7 @@ std::size_t few_rows_limit(unsigned sm_count, std::size_t tiles, std::size_t k, 
 // rows 10.7 / 11.0; a SwiGLU still 13.3 / 12.3 at 208) and with a float32 update (8192 x 2560 160 rows 17.5 / 17.5, 5120 x 2560 208 rows 16.6 / 15.4,
 // 5120 x 1024 160 rows 10.6 / 11.0; in more parts 2560 x 1024 256 rows 10.0 / 11.1).
 bool few_rows_wins(unsigned sm_count, std::size_t t, std::size_t n, std::size_t k, bool int8, Epilogue epilogue, bool float_rows) {
-    const bool add = epilogue == Epilogue::Add, reduced = add && float_rows;  // (float_rows: float32 in 16-byte aligned rows)
+    const bool add = epilogue == Epilogue::Add, reduced = add && float_rows;  // (float_rows: float32 rows that the TMA takes)
     if (t <= kBM) return int8 || t <= few_rows_limit(sm_count, (n + 127) / 128, k, epilogue, reduced);
     if (t > kFewMaxRows || k < 1024) return false;  // (a k loop of a dozen steps has nothing to share)
     const unsigned split = few_schedule(sm_count, t, n, k, int8).split;
@@ -2861,7 +2870,7 @@ GemmParams common_params(Context& ctx, void* y, std::size_t ld_y, bool y_half, s
     p.counters = ctx.scratch.tile_counters;
     p.status = ctx.status;
     // The residual update of the float32 stream goes through shared memory and a TMA reduce-add when Y can be described to the TMA.
-    p.staged_add = (epilogue == Epilogue::Add && !y_half && p.vec_ok != 0) ? 2u : 0u;
+    p.staged_add = (epilogue == Epilogue::Add && !y_half && tma_takes_rows(p)) ? 2u : 0u;
     p.issuers = 1;
     p.early_w = ctx.static_weights ? 1u : 0u;
     return p;
@@ -2898,7 +2907,7 @@ void launch_gemm_f16(Context& ctx, const void* x, std::size_t ld_x, const void* 
     require_aligned(w, "W");
     check(cudaSetDevice(ctx.device), "cudaSetDevice");
     const FewCall few{x, ld_x, w, ld_w, false, nullptr, 0, nullptr, nullptr, y, ld_y, y_half, t, n, k, epilogue};
-    const bool aligned_f32 = !y_half && reinterpret_cast<std::uintptr_t>(y) % 16 == 0 && ld_y % 4 == 0;
+    const bool aligned_f32 = !y_half && tma_takes_rows(y, ld_y, n, false);
     if (config >= kFewConfig || (config == -1 && few_rows_wins(static_cast<unsigned>(ctx.sm_count), t, n, k, false, epilogue, aligned_f32))) {
         launch_few(ctx, few, config, stream);
         return;
@@ -3047,7 +3056,7 @@ void launch_gemm_w8g(Context& ctx, const void* x, std::size_t ld_x, const W8gMat
     require_aligned(x, "X");
     require_aligned(q, "q");
     check(cudaSetDevice(ctx.device), "cudaSetDevice");
-    const bool aligned_f32 = !y_half && reinterpret_cast<std::uintptr_t>(y) % 16 == 0 && ld_y % 4 == 0;
+    const bool aligned_f32 = !y_half && tma_takes_rows(y, ld_y, n, false);
     const bool padded_scales = unit_scales || (ld_st % 8 == 0 && ld_st >= (n + 127) / 128 * 128 && reinterpret_cast<std::uintptr_t>(scales_t) % 16 == 0);
     const FewCall few{x, ld_x, q, ld_q, true, scales_t, ld_st, descale, wm.col_scale, y, ld_y, y_half, t, n, k, epilogue};
     // (above 128 rows every other kernel wants rows padded to 256, as documented: one answer to a caller's table whatever the shape)
@@ -3066,7 +3075,7 @@ void launch_gemm_w8g(Context& ctx, const void* x, std::size_t ld_x, const W8gMat
         if ((swapped < 64 || swapped > 192 || swapped % 32 != 0) && swapped != 256 && swapped != 320)
             throw std::invalid_argument("launch_gemm_w8g: config 512 + w takes w = 64, 96, ..., 192 tokens per tile, or 256 or 320 (two blocks of half as many)");
     } else if (config == -1) {
-        const bool aligned = reinterpret_cast<std::uintptr_t>(y) % 16 == 0 && (ld_y * (y_half ? 2 : 4)) % 16 == 0;
+        const bool aligned = tma_takes_rows(y, ld_y, epilogue == Epilogue::SwiGLU ? n / 2 : n, y_half);
         // whether the result leaves through shared memory and the TMA: all but a float32 SwiGLU and a binary16 residual update
         const bool staged = aligned && (epilogue == Epilogue::Add ? !y_half : (y_half || epilogue != Epilogue::SwiGLU));
         swapped = w8g_swapped_tokens(static_cast<unsigned>(ctx.sm_count), t, n, k, staged, epilogue);

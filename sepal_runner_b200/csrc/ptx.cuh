@@ -97,8 +97,8 @@ __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, uint32
                  : "memory");
 }
 // A box of shared memory stored to the tensor `map` describes, at element coordinates (c0 innermost, c1 rows); what lies outside the
-// tensor is dropped. Asynchronous, grouped and awaited like the reduce above. c0 * element size must be a multiple of 16 bytes; never
-// start at a negative coordinate.
+// tensor is dropped, along a row in units of 16 bytes (as by the reduce above). Asynchronous, grouped and awaited like the reduce. c0 *
+// element size must be a multiple of 16 bytes; never start at a negative coordinate.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int32_t c0, int32_t c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src),
                  "r"(c0), "r"(c1)
