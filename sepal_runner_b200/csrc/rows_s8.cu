@@ -92,11 +92,12 @@ template <bool NORM>
 __device__ __forceinline__ RowScale row_scale(float sum, unsigned top_bits, const RowsParams& p) {
     RowScale s;
     const float top = __uint_as_float(top_bits);
-    s.finite = top_bits < kInfBits && (!NORM || sum < __uint_as_float(kInfBits));  // (a NaN sum compares false)
     s.lift = top < 0x1p-64f ? 0x1p64f : 1.0f;
     s.inv = top > 0.0f ? __fdiv_rn(127.0f, __fmul_rn(top, s.lift)) : 0.0f;
     float scaled = top;
     if constexpr (NORM) scaled = __fdiv_rn(top, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(p.cols)), p.eps)));
+    // max |v| itself: it may overflow where max |u| did not. (NaN compares false; squares that overflow would leave a maximum of 0.)
+    s.finite = scaled < __uint_as_float(kInfBits) && (!NORM || sum < __uint_as_float(kInfBits));
     s.scale = s.finite ? __fdiv_rn(scaled, 127.0f) : __uint_as_float(0x7FC00000u);
     return s;
 }
