@@ -265,7 +265,8 @@ typedef struct sepal_b200_trunk_config {
     uint32_t dn_in, dn_v_offset, dn_v;    /* fused DeltaNet in-projection width; the band its out-projection reads */
     uint32_t max_call_tokens;             /* rows per call; a longer request is cut into calls (gpu_decision_engine.cpp:233-245) */
     uint32_t mlp_int8;                    /* 1: gate_up and down stored as int8 groups; 2: as int8 with one scale an output row, multiplied by
-                                           * int8 activations with one scale a token (the calls under "activations in 8 bits") */
+                                           * int8 activations with one scale a token (the calls under "activations in 8 bits"; eps then at
+                                           * least 1e-30); other values are refused */
     float eps;
     uint64_t seed;
     uint32_t attn_o;                      /* width the attention out-projection reads; 0: attn_q (a real q_proj also carries the output gate) */

@@ -378,11 +378,13 @@ void check_rows(const char* who, std::size_t rows, std::size_t cols, std::size_t
 
 }  // namespace
 
+bool norm_s8_takes_eps(float eps) { return eps >= 1.0e-30f && std::isfinite(eps); }
+
 void launch_rms_norm_s8(const Context& ctx, float* x, std::size_t ld_x, const void* delta, std::size_t ld_delta, bool delta_half, const float* w, const float* col_scale,
                         std::int8_t* q, std::size_t ld_q, float* scales, void* values, std::size_t ld_values, std::size_t rows, std::size_t cols, float eps, cudaStream_t stream) {
     check_rows("launch_rms_norm_s8", rows, cols, ld_x, ld_q, values, ld_values);
     if (delta != nullptr && ld_delta < cols) throw std::invalid_argument("launch_rms_norm_s8: the stride of delta does not hold a row");
-    if (!(eps >= 1.0e-30f) || !std::isfinite(eps)) throw std::invalid_argument("launch_rms_norm_s8: eps must be a positive number (1e-30 at least)");
+    if (!norm_s8_takes_eps(eps)) throw std::invalid_argument("launch_rms_norm_s8: eps must be a positive number (1e-30 at least)");
     if (rows == 0) return;
     if (x == nullptr || w == nullptr || q == nullptr || scales == nullptr) throw std::invalid_argument("launch_rms_norm_s8: null pointer");
     if (!aligned(x, 4) || !aligned(w, 4) || !aligned(scales, 4) || !aligned(col_scale, 4) || !aligned(delta, delta_half ? 2 : 4) || !aligned(values, 2))

@@ -21,6 +21,9 @@ namespace sepal::b200 {
 void launch_rms_norm_s8(const Context& ctx, float* x, std::size_t ld_x, const void* delta, std::size_t ld_delta, bool delta_half, const float* w, const float* col_scale,
                         std::int8_t* q, std::size_t ld_q, float* scales, void* values, std::size_t ld_values, std::size_t rows, std::size_t cols, float eps, cudaStream_t stream);
 
+/// The eps that launch_rms_norm_s8 takes: 1e-30 or more, and finite.
+bool norm_s8_takes_eps(float eps);
+
 /// The quantisation alone, for activations that no norm makes: v = x * col_scale, then as above. x binary16 (x_half) or float32. On
 /// binary16 rows of finite values the bits are those of launch_quantize_rows_s8 (with a col_scale, where the largest product is 2^-121 or more
 /// or zero: below that the other's factor 127 / max overflows).

@@ -129,6 +129,7 @@ private:
     bool real_attention() const { return cfg_.attn_heads != 0; }
     bool real_deltanet() const { return cfg_.dn_value_heads != 0; }
     bool mlp_s8() const { return cfg_.mlp_int8 == 2; }  // int8 activations and int8 weights, integer products
+    static TrunkConfig checked(TrunkConfig config);
     DeltaNetShape deltanet_shape() const;
 
     TrunkConfig cfg_;
