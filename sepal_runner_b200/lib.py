@@ -122,8 +122,8 @@ def pack_gate_up_source(p: int, inter: int) -> int:
 
 
 def _stream_ptr(stream) -> int:
-    """The cudaStream_t of `stream`, or of the current stream of the current device. The latter is asked for as a number where this torch
-    has a way to (torch.cuda.current_stream() builds a Stream object, 3.3 us of host time a launch)."""
+    """The cudaStream_t of `stream`, or of the current stream of the current device: the rule of a call without a Context. The latter is
+    asked for as a number where this torch has a way to (torch.cuda.current_stream() builds a Stream object, 3.3 us of host time a launch)."""
     if stream is not None:
         return int(stream.cuda_stream)
     import torch
@@ -132,7 +132,7 @@ def _stream_ptr(stream) -> int:
     return int(torch.cuda.current_stream().cuda_stream) if raw is None else raw(torch.cuda.current_device())
 
 
-# torch and what the 8-bit calls ask of it at every call, looked up once (_torch): at one token the checks of a call are what it costs.
+# torch and what a Context's calls ask of it every time, looked up once (_torch): at one token the checks of a call are what it costs.
 _TORCH = _I8 = _F16 = _F32 = _RAW_STREAM = None
 
 
@@ -174,7 +174,8 @@ class W8gWeight:
 
 
 class Context:
-    """Per-device state + the launchers. All tensors are CUDA tensors of the context's device; launches go to the current stream."""
+    """Per-device state + the launchers. All tensors are CUDA tensors of the context's device; launches go to `stream`, or to the current
+    stream of the context's device."""
 
     def __init__(self, device: int = 0, workspace_bytes: int = 0) -> None:
         self._lib = library()
@@ -194,6 +195,21 @@ class Context:
         except Exception:
             pass
 
+    def _stream(self, stream) -> int:
+        """The cudaStream_t of `stream` (a torch stream of the context's device), or of the current stream of that device, which need not be
+        the current one."""
+        if stream is not None:
+            if stream.device.index != self.device:
+                raise ValueError(f"the stream is one of {stream.device}, the context is on cuda:{self.device}")
+            return int(stream.cuda_stream)
+        if _TORCH is None:
+            _torch()
+        return _RAW_STREAM(self.device) if _RAW_STREAM is not None else int(_TORCH.cuda.current_stream(self.device).cuda_stream)
+
+    def _here(self):
+        """The context's device as the current one: for the calls of the library that take no context and so run on the current device."""
+        return _torch().cuda.device(self.device)
+
     def info(self) -> dict:
         needed = _u64()
         self._lib.sepal_b200_info(self._h, None, 0, C.byref(needed))
@@ -204,7 +220,7 @@ class Context:
     def status(self, stream=None) -> int:
         """Waits for the stream, returns and clears the device status word (0 = every kernel ran to completion)."""
         out = _i32()
-        _check(self._lib.sepal_b200_status(self._h, _stream_ptr(stream), C.byref(out)))
+        _check(self._lib.sepal_b200_status(self._h, self._stream(stream), C.byref(out)))
         return out.value
 
     def set_static_weights(self, on: bool = True) -> None:
@@ -214,7 +230,7 @@ class Context:
 
     def debug_leave_status(self, code: int, stale_counters: int = 0, stream=None) -> None:
         """Leaves the context as a kernel that gave up waiting would (sepal_b200_debug_leave_status): for tests of the recovery path."""
-        _check(self._lib.sepal_b200_debug_leave_status(self._h, _stream_ptr(stream), code, stale_counters))
+        _check(self._lib.sepal_b200_debug_leave_status(self._h, self._stream(stream), code, stale_counters))
 
     def check_status(self, stream=None) -> None:
         st = self.status(stream)
@@ -250,7 +266,7 @@ class Context:
         y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half)
         _check(self._lib.sepal_b200_gemm_f16(self._h, x.data_ptr(), x.stride(0) if t > 1 else max(x.stride(0), k), w.data_ptr(),
                                              w.stride(0) if n > 1 else max(w.stride(0), k), y.data_ptr(), y.stride(0) if t > 1 else y.shape[1],
-                                             1 if y_half else 0, t, n, k, epilogue, config, _stream_ptr(stream)))
+                                             1 if y_half else 0, t, n, k, epilogue, config, self._stream(stream)))
         return y
 
     def quantize_group_s8(self, w32, stream=None):
@@ -261,7 +277,8 @@ class Context:
         n, k = w32.shape
         q = torch.empty((n, k), dtype=torch.int8, device=w32.device)
         s = torch.empty((n, k // GROUP), dtype=torch.float32, device=w32.device)
-        _check(self._lib.sepal_b200_quantize_group_s8(w32.data_ptr(), k, q.data_ptr(), k, s.data_ptr(), k // GROUP, n, k, _stream_ptr(stream)))
+        with self._here():
+            _check(self._lib.sepal_b200_quantize_group_s8(w32.data_ptr(), k, q.data_ptr(), k, s.data_ptr(), k // GROUP, n, k, self._stream(stream)))
         return q, s
 
     def prepare_w8g(self, q, s, stream=None) -> W8gWeight:
@@ -275,8 +292,9 @@ class Context:
         ld_st = (n + 255) // 256 * 256  # rows padded to whole tiles (zeros): the kernels copy a tile's scales in 16-byte pieces
         st = torch.zeros((groups, ld_st), dtype=torch.float16, device=q.device)
         descale = torch.empty((2,), dtype=torch.float32, device=q.device)  # [0] the factor, [1] scratch for the maximum
-        _check(self._lib.sepal_b200_prepare_w8g_scales(s.data_ptr(), groups, n, groups, st.data_ptr(), ld_st, descale.data_ptr(),
-                                                       descale.data_ptr() + 4, _stream_ptr(stream)))
+        with self._here():
+            _check(self._lib.sepal_b200_prepare_w8g_scales(s.data_ptr(), groups, n, groups, st.data_ptr(), ld_st, descale.data_ptr(),
+                                                           descale.data_ptr() + 4, self._stream(stream)))
         return W8gWeight(q=q, scales=s, scales_t=st, descale=descale)
 
     def gemm_w8g(self, x, w: W8gWeight, y=None, *, epilogue: int = STORE, y_half: bool = True, config: int = -1, stream=None):
@@ -293,7 +311,7 @@ class Context:
         y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half)
         _check(self._lib.sepal_b200_gemm_w8g(self._h, x.data_ptr(), x.stride(0) if t > 1 else max(x.stride(0), k), w.q.data_ptr(), w.q.stride(0),
                                              w.scales_t.data_ptr(), w.scales_t.stride(0), w.descale.data_ptr(), y.data_ptr(),
-                                             y.stride(0) if t > 1 else y.shape[1], 1 if y_half else 0, t, n, k, epilogue, config, _stream_ptr(stream)))
+                                             y.stride(0) if t > 1 else y.shape[1], 1 if y_half else 0, t, n, k, epilogue, config, self._stream(stream)))
         return y
 
     def quantize_rows_s8(self, w16, col_scale=None, stream=None):
@@ -306,8 +324,9 @@ class Context:
         sw = torch.empty((n,), dtype=torch.float32, device=w16.device)
         if col_scale is not None:
             assert col_scale.dtype == torch.float32 and col_scale.is_contiguous() and col_scale.numel() == k
-        _check(self._lib.sepal_b200_quantize_rows_s8(w16.data_ptr(), k, q.data_ptr(), k, sw.data_ptr(), n, k,
-                                                     col_scale.data_ptr() if col_scale is not None else None, _stream_ptr(stream)))
+        with self._here():
+            _check(self._lib.sepal_b200_quantize_rows_s8(w16.data_ptr(), k, q.data_ptr(), k, sw.data_ptr(), n, k,
+                                                         col_scale.data_ptr() if col_scale is not None else None, self._stream(stream)))
         return q, sw
 
     def gemm_w8r(self, x, q, sw, y=None, *, epilogue: int = STORE, y_half: bool = True, config: int = -1, stream=None):
@@ -324,25 +343,19 @@ class Context:
         y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half)
         _check(self._lib.sepal_b200_gemm_w8r(self._h, x.data_ptr(), x.stride(0) if t > 1 else max(x.stride(0), k), q.data_ptr(), q.stride(0),
                                              sw.data_ptr(), y.data_ptr(), y.stride(0) if t > 1 else y.shape[1], 1 if y_half else 0, t, n, k,
-                                             epilogue, config, _stream_ptr(stream)))
+                                             epilogue, config, self._stream(stream)))
         return y
 
     # ---- activations in 8 bits ---------------------------------------------------------------------------------------------
     # Each call asks what the C ABI cannot see in one expression; only a call that fails it is taken apart for the message. A lone row's stride,
     # to which torch may give any value, is never used: the row's length goes in its place.
-    def _stream(self, stream) -> int:
-        """The cudaStream_t of `stream`, or of the current stream of the context's device (which need not be the current one)."""
-        if stream is not None:
-            return int(stream.cuda_stream)
-        return _RAW_STREAM(self.device) if _RAW_STREAM is not None else int(_torch().cuda.current_stream(self.device).cuda_stream)
-
-    def _rows_call(self, call, who: str, head, t: int, c: int, q, scales, col_scale, values, tail, stream):
+    def _rows_call(self, call, who: str, x, head, q, scales, col_scale, values, tail, stream):
         """What the two calls that leave int8 rows have in common: q and scales (new ones, q in rows of a multiple of 16 bytes as gemm_s8
         takes them, or the caller's), col_scale and values checked, and the call."""
-        device = self.device
+        device, (t, c) = self.device, x.shape
         if q is None:
             ld_q = (c + 15) // 16 * 16
-            q = _TORCH.empty((t, ld_q), dtype=_I8, device=f"cuda:{device}")[:, :c]
+            q = _TORCH.empty((t, ld_q), dtype=_I8, device=x.device)[:, :c]
         else:
             if q.dtype is not _I8 or q.get_device() != device or q.shape != (t, c):
                 _require_matrix(who, "q", q, (_I8,), device, t, c)
@@ -352,7 +365,7 @@ class Context:
             if t < 2:
                 ld_q = c
         if scales is None:
-            scales = _TORCH.empty((t,), dtype=_F32, device=f"cuda:{device}")
+            scales = _TORCH.empty((t,), dtype=_F32, device=x.device)
         elif scales.dtype is not _F32 or scales.get_device() != device or scales.numel() != t or not scales.is_contiguous():
             _require_vector(who, "scales", scales, t, device)
         smooth, stands, ld_stands = None, None, 0
@@ -394,8 +407,8 @@ class Context:
         if delta is not None:
             _require_matrix("rms_norm_s8", "delta", delta, (_F16, _F32), device, t, c)
             added, ld_added, half = delta.data_ptr(), delta.stride(0) if t > 1 else c, 1 if delta.dtype is _F16 else 0
-        return self._rows_call(self._lib.sepal_b200_rms_norm_s8, "rms_norm_s8", (x.data_ptr(), ld_x, added, ld_added, half, w.data_ptr()), t, c, q, scales, col_scale,
-                               values, (eps,), stream)
+        return self._rows_call(self._lib.sepal_b200_rms_norm_s8, "rms_norm_s8", x, (x.data_ptr(), ld_x, added, ld_added, half, w.data_ptr()), q, scales, col_scale, values,
+                               (eps,), stream)
 
     def quantize_tokens_s8(self, x, q=None, scales=None, *, col_scale=None, values=None, stream=None):
         """One int8 row with a float32 scale a token (sepal_b200_quantize_tokens_s8): x float16 or float32 [T, K] (times col_scale, float32
@@ -411,8 +424,8 @@ class Context:
             _require_matrix("quantize_tokens_s8", "x", x, (_F16, _F32), device)
         if t < 2:
             ld_x = k
-        return self._rows_call(self._lib.sepal_b200_quantize_tokens_s8, "quantize_tokens_s8", (x.data_ptr(), ld_x, 1 if kind is _F16 else 0), t, k, q, scales, col_scale,
-                               values, (), stream)
+        return self._rows_call(self._lib.sepal_b200_quantize_tokens_s8, "quantize_tokens_s8", x, (x.data_ptr(), ld_x, 1 if kind is _F16 else 0), q, scales, col_scale, values, (),
+                               stream)
 
     def gemm_s8(self, xq, sx, wq, sw, y=None, *, epilogue: int = STORE, y_half: bool = True, config: int = -1, stream=None):
         """y = epilogue(float(xq @ wq.T) * sx[:, None] * sw): xq int8 [T, K] with sx float32 [T] (rms_norm_s8, quantize_tokens_s8), wq int8
@@ -468,14 +481,16 @@ class Context:
         rows, cols = stacked.shape
         out = torch.empty_like(stacked)
         nbytes = cols * stacked.element_size()
-        _check(self._lib.sepal_b200_pack_gate_up(stacked.data_ptr(), nbytes, out.data_ptr(), nbytes, rows // 2, nbytes, _stream_ptr(stream)))
+        with self._here():
+            _check(self._lib.sepal_b200_pack_gate_up(stacked.data_ptr(), nbytes, out.data_ptr(), nbytes, rows // 2, nbytes, self._stream(stream)))
         return out
 
     def float_to_half(self, src, stream=None):
         import torch
 
         dst = torch.empty(src.shape, dtype=torch.float16, device=src.device)
-        _check(self._lib.sepal_b200_float_to_half(src.data_ptr(), dst.data_ptr(), src.numel(), _stream_ptr(stream)))
+        with self._here():
+            _check(self._lib.sepal_b200_float_to_half(src.data_ptr(), dst.data_ptr(), src.numel(), self._stream(stream)))
         return dst
 
     @staticmethod
@@ -504,7 +519,7 @@ def attention_prepare(ctx, shape, rows, q_gate, k, v, q_norm, k_norm, q_out, k_a
     half = lambda t: 1 if t.dtype == torch.float16 else 0  # noqa: E731
     _check(ctx._lib.sepal_b200_attention_prepare(ctx._h, C.byref(shape), table, len(rows), q_gate.data_ptr(), q_gate.stride(0), half(q_gate), k.data_ptr(),
                                                  k.stride(0), half(k), v.data_ptr(), v.stride(0), half(v), q_norm.data_ptr(), k_norm.data_ptr(),
-                                                 q_out.data_ptr(), q_out.stride(0), k_arena.data_ptr(), v_arena.data_ptr(), k_arena.shape[0], _stream_ptr(stream)))
+                                                 q_out.data_ptr(), q_out.stride(0), k_arena.data_ptr(), v_arena.data_ptr(), k_arena.shape[0], ctx._stream(stream)))
 
 
 def attention(ctx, shape, rows, q, k_arena, v_arena, gate, out, stream=None):
@@ -514,7 +529,7 @@ def attention(ctx, shape, rows, q, k_arena, v_arena, gate, out, stream=None):
     table = (AttentionRow * len(rows))(*[AttentionRow(*r) for r in rows])
     _check(ctx._lib.sepal_b200_attention(ctx._h, C.byref(shape), table, len(rows), q.shape[0], q.data_ptr(), q.stride(0), k_arena.data_ptr(), v_arena.data_ptr(),
                                          k_arena.shape[0], gate.data_ptr(), gate.stride(0), 1 if gate.dtype == torch.float16 else 0, out.data_ptr(),
-                                         out.stride(0), _stream_ptr(stream)))
+                                         out.stride(0), ctx._stream(stream)))
 
 
 class DeltaNetShape(C.Structure):
@@ -542,7 +557,7 @@ def deltanet(ctx, shape, rows, mixed, z, b, a, conv, a_log, dt_bias, norm, state
     _check(ctx._lib.sepal_b200_deltanet(ctx._h, C.byref(shape), table, len(rows), mixed.data_ptr(), mixed.stride(0), z.data_ptr(), z.stride(0), b.data_ptr(),
                                         b.stride(0), a.data_ptr(), a.stride(0), 1 if mixed.dtype == torch.float16 else 0, conv.data_ptr(), a_log.data_ptr(),
                                         dt_bias.data_ptr(), norm.data_ptr(), scratch.data_ptr(), states.data_ptr(), tails.data_ptr(), states.shape[0],
-                                        out.data_ptr(), out.stride(0), _stream_ptr(stream)))
+                                        out.data_ptr(), out.stride(0), ctx._stream(stream)))
     return scratch  # kept alive by the caller until the stream has run
 
 

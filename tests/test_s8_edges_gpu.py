@@ -74,3 +74,13 @@ def test_rows_that_the_weights_quantiser_treats_otherwise(ctx):
     x[2, 3], x[3, 5] = float("nan"), float("inf")
     q, s = ctx.quantize_tokens_s8(x)
     assert torch.isnan(s).tolist() == [False, False, True, True] and (q[2:] == 0).all()
+
+
+def test_a_context_before_torch_has_touched_the_gpu():
+    """The stream of a call is found in a process whose torch has not initialised CUDA yet."""
+    import os
+    import subprocess
+    import sys
+
+    code = "import sepal_runner_b200 as sb; c = sb.Context(0); assert c.status() == 0; c.debug_leave_status(5); assert c.status() == 5 and c.status() == 0; c.close()"
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
