@@ -147,6 +147,15 @@ def _torch():
     return _TORCH
 
 
+def _empty(shape, dtype, device, stream):
+    """A new tensor for a call on `stream` (None: the current one): one of that stream's, as torch's allocator counts them. Memory taken on the
+    current stream may still be in use by work there, and goes back to it when the tensor is dropped, while the call's own stream runs on."""
+    if stream is None:
+        return _torch().empty(shape, dtype=dtype, device=device)
+    with _torch().cuda.stream(stream):
+        return _TORCH.empty(shape, dtype=dtype, device=device)
+
+
 def _require_matrix(who: str, what: str, t, dtypes, device: int, rows=None, columns=None) -> None:
     """Raises unless t is a [rows, columns] (None: any) matrix of one of `dtypes` on cuda:`device` whose rows are contiguous."""
     shape = tuple(t.shape)
@@ -175,7 +184,7 @@ class W8gWeight:
 
 class Context:
     """Per-device state + the launchers. All tensors are CUDA tensors of the context's device; launches go to `stream`, or to the current
-    stream of the context's device."""
+    stream of the context's device. What a call allocates for its results belongs to the stream that it was launched on."""
 
     def __init__(self, device: int = 0, workspace_bytes: int = 0) -> None:
         self._lib = library()
@@ -239,13 +248,13 @@ class Context:
 
     # ---- launchers -------------------------------------------------------------------------------------------------------
     @staticmethod
-    def _out(x, n_out: int, y, y_half: bool):
+    def _out(x, n_out: int, y, y_half: bool, stream=None):
         """The output tensor: a new one, or the caller's after checking that the C ABI (which only sees a pointer and a row stride) would
         write inside it: [T, n_out], float16 or float32, on x's device, last dimension contiguous."""
         import torch
 
         if y is None:
-            return torch.empty((x.shape[0], n_out), dtype=torch.float16 if y_half else torch.float32, device=x.device)
+            return _empty((x.shape[0], n_out), torch.float16 if y_half else torch.float32, x.device, stream)
         if tuple(y.shape) != (x.shape[0], n_out):
             raise ValueError(f"the output must be [{x.shape[0]}, {n_out}], not {tuple(y.shape)}")
         if y.dtype not in (torch.float16, torch.float32) or y.device != x.device or (y.numel() > 0 and y.stride(-1) != 1):
@@ -263,7 +272,7 @@ class Context:
             raise ValueError(f"x is [{t}, {k}] but w is {tuple(w.shape)} on {w.device}: the inner dimensions and the devices must agree")
         if y is not None:
             y_half = y.dtype == torch.float16
-        y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half)
+        y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half, stream)
         _check(self._lib.sepal_b200_gemm_f16(self._h, x.data_ptr(), x.stride(0) if t > 1 else max(x.stride(0), k), w.data_ptr(),
                                              w.stride(0) if n > 1 else max(w.stride(0), k), y.data_ptr(), y.stride(0) if t > 1 else y.shape[1],
                                              1 if y_half else 0, t, n, k, epilogue, config, self._stream(stream)))
@@ -275,8 +284,8 @@ class Context:
 
         assert w32.dtype == torch.float32 and w32.is_contiguous()
         n, k = w32.shape
-        q = torch.empty((n, k), dtype=torch.int8, device=w32.device)
-        s = torch.empty((n, k // GROUP), dtype=torch.float32, device=w32.device)
+        q = _empty((n, k), torch.int8, w32.device, stream)
+        s = _empty((n, k // GROUP), torch.float32, w32.device, stream)
         with self._here():
             _check(self._lib.sepal_b200_quantize_group_s8(w32.data_ptr(), k, q.data_ptr(), k, s.data_ptr(), k // GROUP, n, k, self._stream(stream)))
         return q, s
@@ -290,8 +299,10 @@ class Context:
         groups = k // GROUP
         assert s.shape == (n, groups)
         ld_st = (n + 255) // 256 * 256  # rows padded to whole tiles (zeros): the kernels copy a tile's scales in 16-byte pieces
-        st = torch.zeros((groups, ld_st), dtype=torch.float16, device=q.device)
-        descale = torch.empty((2,), dtype=torch.float32, device=q.device)  # [0] the factor, [1] scratch for the maximum
+        st = _empty((groups, ld_st), torch.float16, q.device, stream)
+        with torch.cuda.stream(stream):  # (None: the current one)
+            st.zero_()
+        descale = _empty((2,), torch.float32, q.device, stream)  # [0] the factor, [1] scratch for the maximum
         with self._here():
             _check(self._lib.sepal_b200_prepare_w8g_scales(s.data_ptr(), groups, n, groups, st.data_ptr(), ld_st, descale.data_ptr(),
                                                            descale.data_ptr() + 4, self._stream(stream)))
@@ -308,7 +319,7 @@ class Context:
             raise ValueError(f"x is [{t}, {k}] but the weights are {tuple(w.q.shape)} on {w.q.device}: the inner dimensions and the devices must agree")
         if y is not None:
             y_half = y.dtype == torch.float16
-        y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half)
+        y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half, stream)
         _check(self._lib.sepal_b200_gemm_w8g(self._h, x.data_ptr(), x.stride(0) if t > 1 else max(x.stride(0), k), w.q.data_ptr(), w.q.stride(0),
                                              w.scales_t.data_ptr(), w.scales_t.stride(0), w.descale.data_ptr(), y.data_ptr(),
                                              y.stride(0) if t > 1 else y.shape[1], 1 if y_half else 0, t, n, k, epilogue, config, self._stream(stream)))
@@ -320,8 +331,8 @@ class Context:
 
         assert w16.dtype == torch.float16 and w16.is_contiguous()
         n, k = w16.shape
-        q = torch.empty((n, k), dtype=torch.int8, device=w16.device)
-        sw = torch.empty((n,), dtype=torch.float32, device=w16.device)
+        q = _empty((n, k), torch.int8, w16.device, stream)
+        sw = _empty((n,), torch.float32, w16.device, stream)
         if col_scale is not None:
             assert col_scale.dtype == torch.float32 and col_scale.is_contiguous() and col_scale.numel() == k
         with self._here():
@@ -340,7 +351,7 @@ class Context:
             raise ValueError(f"x is [{t}, {k}], q is {tuple(q.shape)}, sw has {sw.numel()} scales: the shapes and the devices must agree")
         if y is not None:
             y_half = y.dtype == torch.float16
-        y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half)
+        y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half, stream)
         _check(self._lib.sepal_b200_gemm_w8r(self._h, x.data_ptr(), x.stride(0) if t > 1 else max(x.stride(0), k), q.data_ptr(), q.stride(0),
                                              sw.data_ptr(), y.data_ptr(), y.stride(0) if t > 1 else y.shape[1], 1 if y_half else 0, t, n, k,
                                              epilogue, config, self._stream(stream)))
@@ -355,7 +366,7 @@ class Context:
         device, (t, c) = self.device, x.shape
         if q is None:
             ld_q = (c + 15) // 16 * 16
-            q = _TORCH.empty((t, ld_q), dtype=_I8, device=x.device)[:, :c]
+            q = _empty((t, ld_q), _I8, x.device, stream)[:, :c]
         else:
             if q.dtype is not _I8 or q.get_device() != device or q.shape != (t, c):
                 _require_matrix(who, "q", q, (_I8,), device, t, c)
@@ -365,7 +376,7 @@ class Context:
             if t < 2:
                 ld_q = c
         if scales is None:
-            scales = _TORCH.empty((t,), dtype=_F32, device=x.device)
+            scales = _empty((t,), _F32, x.device, stream)
         elif scales.dtype is not _F32 or scales.get_device() != device or scales.numel() != t or not scales.is_contiguous():
             _require_vector(who, "scales", scales, t, device)
         smooth, stands, ld_stands = None, None, 0
@@ -457,7 +468,7 @@ class Context:
         if y is None:
             if epilogue == ADD:
                 raise ValueError("gemm_s8: epilogue ADD updates an output that the caller gives")
-            y, ld_y = _TORCH.empty((t, columns), dtype=_F16 if y_half else _F32, device=xq.device), columns
+            y, ld_y = _empty((t, columns), _F16 if y_half else _F32, xq.device, stream), columns
         else:
             kind = y.dtype
             y_half = kind is _F16
@@ -475,20 +486,16 @@ class Context:
 
     def pack_gate_up(self, stacked, stream=None):
         """[gate; up] (2 I rows) -> the packed row order of the fused SwiGLU multiply."""
-        import torch
-
         assert stacked.is_contiguous()
         rows, cols = stacked.shape
-        out = torch.empty_like(stacked)
+        out = _empty(stacked.shape, stacked.dtype, stacked.device, stream)
         nbytes = cols * stacked.element_size()
         with self._here():
             _check(self._lib.sepal_b200_pack_gate_up(stacked.data_ptr(), nbytes, out.data_ptr(), nbytes, rows // 2, nbytes, self._stream(stream)))
         return out
 
     def float_to_half(self, src, stream=None):
-        import torch
-
-        dst = torch.empty(src.shape, dtype=torch.float16, device=src.device)
+        dst = _empty(src.shape, _torch().float16, src.device, stream)
         with self._here():
             _check(self._lib.sepal_b200_float_to_half(src.data_ptr(), dst.data_ptr(), src.numel(), self._stream(stream)))
         return dst
@@ -552,7 +559,7 @@ def deltanet(ctx, shape, rows, mixed, z, b, a, conv, a_log, dt_bias, norm, state
     table = (DeltaNetRow * len(rows))(*[DeltaNetRow(*r) for r in rows])
     n = max((r[0] + r[1] for r in rows), default=0)
     kd, vd = shape.key_heads * shape.head_dim, shape.value_heads * shape.head_dim
-    scratch = torch.empty(max(1, n * (264 * shape.key_heads + 2 * vd + 58 * shape.value_heads)), dtype=torch.float32, device=out.device)
+    scratch = _empty(max(1, n * (264 * shape.key_heads + 2 * vd + 58 * shape.value_heads)), torch.float32, out.device, stream)
     assert mixed.dtype == z.dtype == b.dtype == a.dtype
     _check(ctx._lib.sepal_b200_deltanet(ctx._h, C.byref(shape), table, len(rows), mixed.data_ptr(), mixed.stride(0), z.data_ptr(), z.stride(0), b.data_ptr(),
                                         b.stride(0), a.data_ptr(), a.stride(0), 1 if mixed.dtype == torch.float16 else 0, conv.data_ptr(), a_log.data_ptr(),

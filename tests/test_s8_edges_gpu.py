@@ -84,3 +84,56 @@ def test_a_context_before_torch_has_touched_the_gpu():
 
     code = "import sepal_runner_b200 as sb; c = sb.Context(0); assert c.status() == 0; c.debug_leave_status(5); assert c.status() == 5 and c.status() == 0; c.close()"
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def stream_of(tensor):
+    """The stream that torch's allocator has a tensor's memory down for."""
+    for segment in torch.cuda.memory_snapshot():
+        if segment["address"] <= tensor.data_ptr() < segment["address"] + segment["total_size"]:
+            return segment["stream"]
+    raise AssertionError("not memory of torch's allocator")
+
+
+def test_results_belong_to_the_stream_of_the_call(ctx):
+    """What a call with `stream=` allocates is that stream's: memory of the current stream may still be in use there, and would be handed
+    out again there while the call's own stream writes it."""
+    side = torch.cuda.Stream()
+    gen = generator(12)
+    x16, x32, w16 = randn(gen, 40, 256).half(), randn(gen, 40, 256), randn(gen, 128, 256).half()
+    gain, stacked = torch.zeros(256, device="cuda"), randn(gen, 128, 256).half()
+    torch.cuda.synchronize()
+    for stream, number in ((side, side.cuda_stream), (None, torch.cuda.current_stream().cuda_stream)):
+        q, s = ctx.rms_norm_s8(x32, gain, stream=stream)
+        q2, s2 = ctx.quantize_tokens_s8(x16, stream=stream)
+        wq, sw = ctx.quantize_rows_s8(w16, stream=stream)
+        gq, gs = ctx.quantize_group_s8(x32, stream=stream)
+        placed = ctx.prepare_w8g(gq, gs, stream=stream)
+        results = [q, s, q2, s2, wq, sw, gq, gs, placed.scales_t, placed.descale, ctx.gemm_s8(q, s, wq, sw, stream=stream), ctx.gemm_f16(x16, w16, stream=stream),
+                   ctx.gemm_w8r(x16, wq, sw, stream=stream), ctx.gemm_w8g(x16, placed, stream=stream), ctx.pack_gate_up(stacked, stream=stream),
+                   ctx.float_to_half(x32, stream=stream)]
+        assert [stream_of(r) for r in results] == [number] * len(results)
+        torch.cuda.synchronize()
+    ctx.check_status()
+
+
+def test_results_on_another_stream_over_busy_memory(ctx):
+    """A result is not placed over memory that the current stream's work still reads."""
+    side = torch.cuda.Stream()
+    gen = generator(13)
+    x = randn(gen, 4096, 4096)
+    gain = torch.zeros(4096, device="cuda")
+    want_q, want_s = ctx.rms_norm_s8(x, gain)
+    source = torch.randint(0, 100, (4096, 4096), generator=gen, device="cuda", dtype=torch.int8)
+    total = source.long().sum().item()
+    matrix = randn(gen, 4096, 4096)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        busy = source.clone()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            matrix @ matrix  # the current stream works for a while before it reads `busy`
+        late = busy.long().sum()
+        del busy
+        q, s = ctx.rms_norm_s8(x, gain, stream=side)
+        torch.cuda.synchronize()
+        assert late.item() == total and torch.equal(q, want_q) and torch.equal(s, want_s)
