@@ -215,6 +215,13 @@ class Context:
             _torch()
         return _RAW_STREAM(self.device) if _RAW_STREAM is not None else int(_TORCH.cuda.current_stream(self.device).cuda_stream)
 
+    def _require_here(self, *tensors) -> None:
+        """Raises unless the tensors are on the context's device: the C ABI sees an address only, and a kernel that reads one of another
+        memory ends the process's use of the GPU."""
+        for t in tensors:
+            if t.get_device() != self.device:
+                raise ValueError(f"a tensor is on {t.device}, the context on cuda:{self.device}")
+
     def _here(self):
         """The context's device as the current one: for the calls of the library that take no context and so run on the current device."""
         return _torch().cuda.device(self.device)
@@ -270,6 +277,7 @@ class Context:
         n = w.shape[0]
         if w.shape[1] != k or w.device != x.device:
             raise ValueError(f"x is [{t}, {k}] but w is {tuple(w.shape)} on {w.device}: the inner dimensions and the devices must agree")
+        self._require_here(x)
         if y is not None:
             y_half = y.dtype == torch.float16
         y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half, stream)
@@ -283,6 +291,7 @@ class Context:
         import torch
 
         assert w32.dtype == torch.float32 and w32.is_contiguous()
+        self._require_here(w32)
         n, k = w32.shape
         q = _empty((n, k), torch.int8, w32.device, stream)
         s = _empty((n, k // GROUP), torch.float32, w32.device, stream)
@@ -295,6 +304,7 @@ class Context:
         import torch
 
         assert q.dtype == torch.int8 and s.dtype == torch.float32 and q.is_contiguous() and s.is_contiguous()
+        self._require_here(q, s)
         n, k = q.shape
         groups = k // GROUP
         assert s.shape == (n, groups)
@@ -317,6 +327,7 @@ class Context:
         n = w.q.shape[0]
         if w.q.shape[1] != k or w.q.device != x.device:
             raise ValueError(f"x is [{t}, {k}] but the weights are {tuple(w.q.shape)} on {w.q.device}: the inner dimensions and the devices must agree")
+        self._require_here(x, w.scales_t, w.descale)
         if y is not None:
             y_half = y.dtype == torch.float16
         y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half, stream)
@@ -330,11 +341,13 @@ class Context:
         import torch
 
         assert w16.dtype == torch.float16 and w16.is_contiguous()
+        self._require_here(w16)
         n, k = w16.shape
         q = _empty((n, k), torch.int8, w16.device, stream)
         sw = _empty((n,), torch.float32, w16.device, stream)
         if col_scale is not None:
             assert col_scale.dtype == torch.float32 and col_scale.is_contiguous() and col_scale.numel() == k
+            self._require_here(col_scale)
         with self._here():
             _check(self._lib.sepal_b200_quantize_rows_s8(w16.data_ptr(), k, q.data_ptr(), k, sw.data_ptr(), n, k,
                                                          col_scale.data_ptr() if col_scale is not None else None, self._stream(stream)))
@@ -349,6 +362,7 @@ class Context:
         n = q.shape[0]
         if q.shape[1] != k or sw.numel() != n or q.device != x.device or sw.device != x.device:
             raise ValueError(f"x is [{t}, {k}], q is {tuple(q.shape)}, sw has {sw.numel()} scales: the shapes and the devices must agree")
+        self._require_here(x)
         if y is not None:
             y_half = y.dtype == torch.float16
         y = self._out(x, n // 2 if epilogue == SWIGLU else n, y, y_half, stream)
@@ -487,6 +501,7 @@ class Context:
     def pack_gate_up(self, stacked, stream=None):
         """[gate; up] (2 I rows) -> the packed row order of the fused SwiGLU multiply."""
         assert stacked.is_contiguous()
+        self._require_here(stacked)
         rows, cols = stacked.shape
         out = _empty(stacked.shape, stacked.dtype, stacked.device, stream)
         nbytes = cols * stacked.element_size()
@@ -495,6 +510,8 @@ class Context:
         return out
 
     def float_to_half(self, src, stream=None):
+        assert src.dtype == _torch().float32 and src.is_contiguous()
+        self._require_here(src)
         dst = _empty(src.shape, _torch().float16, src.device, stream)
         with self._here():
             _check(self._lib.sepal_b200_float_to_half(src.data_ptr(), dst.data_ptr(), src.numel(), self._stream(stream)))
@@ -522,6 +539,7 @@ def attention_prepare(ctx, shape, rows, q_gate, k, v, q_norm, k_norm, q_out, k_a
     """Norm, RoPE and cache append (sepal_b200_attention_prepare). rows: list of (q_begin, length, kv_begin, context); torch tensors."""
     import torch
 
+    ctx._require_here(q_gate, k, v, q_norm, k_norm, q_out, k_arena, v_arena)
     table = (AttentionRow * len(rows))(*[AttentionRow(*r) for r in rows])
     half = lambda t: 1 if t.dtype == torch.float16 else 0  # noqa: E731
     _check(ctx._lib.sepal_b200_attention_prepare(ctx._h, C.byref(shape), table, len(rows), q_gate.data_ptr(), q_gate.stride(0), half(q_gate), k.data_ptr(),
@@ -533,6 +551,7 @@ def attention(ctx, shape, rows, q, k_arena, v_arena, gate, out, stream=None):
     """Causal grouped-query flash attention times sigmoid(gate) (sepal_b200_attention)."""
     import torch
 
+    ctx._require_here(q, k_arena, v_arena, gate, out)
     table = (AttentionRow * len(rows))(*[AttentionRow(*r) for r in rows])
     _check(ctx._lib.sepal_b200_attention(ctx._h, C.byref(shape), table, len(rows), q.shape[0], q.data_ptr(), q.stride(0), k_arena.data_ptr(), v_arena.data_ptr(),
                                          k_arena.shape[0], gate.data_ptr(), gate.stride(0), 1 if gate.dtype == torch.float16 else 0, out.data_ptr(),
@@ -556,6 +575,7 @@ def deltanet(ctx, shape, rows, mixed, z, b, a, conv, a_log, dt_bias, norm, state
     dtype (float16 or float32); states [slots, value_heads, 128, 128] and tails [slots, K - 1, conv_dim] float32, updated in place."""
     import torch
 
+    ctx._require_here(mixed, z, b, a, conv, a_log, dt_bias, norm, states, tails, out)
     table = (DeltaNetRow * len(rows))(*[DeltaNetRow(*r) for r in rows])
     n = max((r[0] + r[1] for r in rows), default=0)
     kd, vd = shape.key_heads * shape.head_dim, shape.value_heads * shape.head_dim

@@ -1,4 +1,4 @@
-"""Which stream the binding's calls go to: host arithmetic, with a library that records what it is given."""
+"""Which stream the binding's calls go to, and whose tensors they take: host arithmetic, with a library that records what it is given."""
 import types
 
 import pytest
@@ -112,4 +112,34 @@ def test_a_stream_of_another_device_is_refused(recorded):
                  lambda: ctx.status(stream=wrong), lambda: ctx.gemm_f16(torch.zeros((4, 16)).half(), torch.zeros((8, 16)).half(), torch.zeros(4, 8), stream=wrong)):
         with pytest.raises(ValueError, match="the context is on"):
             call()
+    assert calls == []
+
+
+def test_tensors_of_another_device_are_refused(recorded):
+    """Every launching call with tensors that are not on the context's device: an address that its kernel could not read."""
+    ctx, calls = recorded
+    calls_here = []
+    for _ in every_call(ctx):
+        calls_here.append(calls[-1][0])
+    ctx.device = 0
+    calls.clear()
+    h, f, b = (lambda *shape, d=d: torch.zeros(shape, dtype=d) for d in (torch.float16, torch.float32, torch.int8))
+    placed = sb.W8gWeight(q=b(8, 128), scales=f(8, 1), scales_t=h(1, 256), descale=f(2))
+    attention = sb.AttentionShape(heads=2, kv_heads=1, head_dim=128, rotary_dims=32, rope_theta=1e4, eps=1e-6)
+    deltanet = sb.DeltaNetShape(key_heads=1, value_heads=1, head_dim=128, conv_kernel=4, eps=1e-6)
+    rows = [(0, 4, 0, 0)]
+    for call in (lambda: ctx.gemm_f16(h(4, 128), h(8, 128)), lambda: ctx.quantize_group_s8(f(128, 128)), lambda: ctx.prepare_w8g(b(8, 128), f(8, 1)),
+                 lambda: ctx.gemm_w8g(h(4, 128), placed), lambda: ctx.quantize_rows_s8(h(8, 128)), lambda: ctx.gemm_w8r(h(4, 128), b(8, 128), f(8)),
+                 lambda: ctx.rms_norm_s8(f(4, 128), f(128)), lambda: ctx.quantize_tokens_s8(h(4, 128)), lambda: ctx.gemm_s8(b(4, 128), f(4), b(8, 128), f(8)),
+                 lambda: ctx.pack_gate_up(h(128, 64)), lambda: ctx.float_to_half(f(64)),
+                 lambda: sb.attention_prepare(ctx, attention, rows, h(4, 512), h(4, 128), h(4, 128), f(128), f(128), h(4, 256), h(16, 128), h(16, 128)),
+                 lambda: sb.attention(ctx, attention, rows, h(4, 256), h(16, 128), h(16, 128), h(4, 256), h(4, 256)),
+                 lambda: sb.deltanet(ctx, deltanet, rows, h(4, 384), h(4, 128), h(4, 1), h(4, 1), f(384, 4), f(1), f(1), f(128), f(1, 1, 128, 128), f(1, 3, 384), h(4, 128))):
+        with pytest.raises(ValueError, match="cuda:0"):
+            call()
+    assert calls == [] and len(calls_here) == 16
+    ctx.device = DEVICE
+    for bad in (torch.zeros(8, dtype=torch.float16), torch.zeros(4, 4).t()[:2]):
+        with pytest.raises(AssertionError):
+            ctx.float_to_half(bad)
     assert calls == []
