@@ -12,6 +12,15 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (run with -m gpu on the GPU box)")
 
 
+@pytest.fixture(autouse=True)
+def launches_overlap():
+    """Every test starts with launches that may overlap, whatever the one before it switched off and however it ended."""
+    yield
+    binding = sys.modules.get("sepal_runner_b200.lib")
+    if binding is not None and binding._LIB is not None:
+        binding._LIB.sepal_b200_set_launch_overlap(1)
+
+
 @pytest.fixture(scope="session")
 def oracle():
     from oracle.oracle import Oracle

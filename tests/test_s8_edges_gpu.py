@@ -137,3 +137,34 @@ def test_results_on_another_stream_over_busy_memory(ctx):
         q, s = ctx.rms_norm_s8(x, gain, stream=side)
         torch.cuda.synchronize()
         assert late.item() == total and torch.equal(q, want_q) and torch.equal(s, want_s)
+
+
+# (few rows of a long k: the few-rows kernel with its parts of k; many: pairs. Both request weights ahead of the kernel before them.)
+@pytest.mark.parametrize("t,hidden,inner", [(1, 1024, 4096), (29, 1024, 4096), (200, 1024, 4096), (700, 512, 640)])
+def test_weights_requested_early_change_no_bits(t, hidden, inner):
+    """A layer's MLP many times over, back to back: as dependents and in plain order, with and without the promise of static weights."""
+    gen = generator(t)
+    start, delta, gain = randn(gen, t, hidden, std=2.0), randn(gen, t, hidden, std=0.1).half(), randn(gen, hidden, std=0.2)
+    c = sb.Context(0)
+    gate_up, gate_up_s = c.quantize_rows_s8(randn(gen, 2 * inner, hidden, std=0.02).half())
+    down, down_s = c.quantize_rows_s8(randn(gen, hidden, inner, std=0.02).half())
+    c.close()
+    torch.cuda.synchronize()
+    results = []
+    for overlap in (1, 0):
+        for static in (False, True):
+            sb.library().sepal_b200_set_launch_overlap(overlap)
+            c = sb.Context(0)
+            c.set_static_weights(static)
+            x = start.clone()
+            torch.cuda.synchronize()
+            for _ in range(12):
+                q, s = c.rms_norm_s8(x, gain, delta=delta)
+                a = c.gemm_s8(q, s, gate_up, gate_up_s, epilogue=sb.SWIGLU)
+                q, s = c.quantize_tokens_s8(a)
+                c.gemm_s8(q, s, down, down_s, x, epilogue=sb.ADD)
+            c.check_status()
+            results.append(x)
+            c.close()
+    assert torch.isfinite(results[0]).all() and not torch.equal(results[0], start)
+    assert all(torch.equal(r, results[0]) for r in results[1:])
