@@ -85,13 +85,15 @@ SEPAL_B200_API uint64_t sepal_b200_take_launch_count(void);
 
 /* Process-wide switch, on by default: the GEMM kernels (and the trunk's embedding and norm kernels) are launched as programmatic
  * dependents of the kernel before them in the stream, so a kernel's set-up overlaps the end of the one before it; each of them waits for
- * that kernel to complete before it touches global memory, so results do not change. No counterpart in the reference (whose engine
+ * that kernel to complete before it touches global memory (but for weights under the promise below), so results do not change. No counterpart in the reference (whose engine
  * launches its kernels one after the other, runner/cuda/src/cuda_engine.cpp:1724-1952); off = plain stream order, for comparisons. */
 SEPAL_B200_API void sepal_b200_set_launch_overlap(int32_t on);
 
 /* The caller's promise for the multiplies it launches through `ctx` from now on (on != 0), or its withdrawal (0, the default): the
- * weight matrix of a multiply (w, or q with its scales) is not written by the kernel that runs directly before the multiply in its
- * stream. An inference engine's weights are uploaded once, so every multiply of the reference's engine qualifies
+ * weight matrix of a multiply (w, or q with its scales) is complete before the multiply is enqueued: nothing that still runs or waits
+ * on the device writes it. (That the kernel directly before the multiply does not write it is not enough: that kernel may itself have
+ * started, and let the multiply start, before the ones ahead of it have finished. Wait for the stream once after the weights are
+ * placed.) An inference engine's weights are uploaded once, so every multiply of the reference's engine qualifies
  * (CudaEngine::Impl::gemm, runner/cuda/src/cuda_engine.cpp:1093-1154, reads device copies written at load time, as
  * CudaGemm::upload_weights writes a provider's, runner/cuda/src/cuda_gemm.cpp:389-394). With the promise a kernel launched as a programmatic dependent (see above)
  * requests its first weight tiles while the kernel before it is still finishing, and waits for that kernel only before it touches the

@@ -47,9 +47,10 @@ struct Context {
     void* table = nullptr;        // device memory for the small per-launch tables of the attention kernels (rows, block lists)
     std::size_t table_bytes = 0;
     unsigned table_turn = 0;
-    /// The caller's promise that the weights of a multiply launched through this context are never written by the kernel that runs
-    /// before it in the stream (an inference engine's weights are uploaded once). A kernel may then request its first weight tiles
-    /// before it waits for that kernel (see launch_overlap below). Off unless set.
+    /// The caller's promise that the weights of a multiply launched through this context are complete before it is enqueued (an inference
+    /// engine's weights are uploaded once, and waited for). A kernel may then request its first weight tiles before it waits for the
+    /// kernels ahead of it (see launch_overlap below): not only the one directly before may still be running then, because that one, too,
+    /// lets its successor start before it has waited for its own predecessor. Off unless set.
     bool static_weights = false;
 
     Context(int device, std::size_t workspace_bytes);

@@ -27,7 +27,7 @@
 // both parts are added to Y by the TMA's reduce-add, the owner of a tile starts its adds only after the tile's counter shows the spare
 // pair's adds performed: Y is (Y + first part) + second part whatever the timing, and nothing is fixed up.
 //
-// With the caller's promise that the weights are not written by the kernel before (Context::static_weights), every kernel requests the
+// With the caller's promise that the weights are complete before the launch is enqueued (Context::static_weights), every kernel requests the
 // weight tiles of its first stages before griddepcontrol.wait and only the activations after it.
 //
 // Every wait on an mbarrier is bounded: when it runs out the CTA raises a flag in shared memory, records a code in the context's

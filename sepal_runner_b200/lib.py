@@ -240,8 +240,9 @@ class Context:
         return out.value
 
     def set_static_weights(self, on: bool = True) -> None:
-        """Promises (or withdraws the promise) that no kernel directly before a multiply of this context writes that multiply's weights
-        (sepal_b200_set_static_weights): the kernels then request their first weight tiles before they wait for the kernel before them."""
+        """Promises (or withdraws the promise) that the weights of every multiply of this context are complete before it is enqueued: placed,
+        and waited for (sepal_b200_set_static_weights). The kernels then request their first weight tiles before they wait for the
+        kernels ahead of them."""
         _check(self._lib.sepal_b200_set_static_weights(self._h, 1 if on else 0))
 
     def debug_leave_status(self, code: int, stale_counters: int = 0, stream=None) -> None:
