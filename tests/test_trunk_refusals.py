@@ -23,8 +23,14 @@ def test_an_eps_that_the_norm_to_bytes_does_not_take(eps):
         sb.Trunk(0, config(mlp_int8=2, eps=eps))
 
 
+def test_widths_whose_sums_do_not_fit():
+    for bad in (dict(hidden=1 << 17), dict(intermediate=1 << 17)):
+        with pytest.raises(sb.SepalB200Error, match="at most 131071"):
+            sb.Trunk(0, config(mlp_int8=2, **bad))
+
+
 def test_widths():
-    for bad in (dict(hidden=200), dict(intermediate=100), dict(dn_v=64), dict(layers=0), dict(dn_v_offset=448), dict(dn_value_heads=1, dn_key_heads=1)):
+    for bad in (dict(hidden=200), dict(hidden=0), dict(intermediate=100), dict(intermediate=0), dict(dn_v=64), dict(layers=0), dict(dn_v_offset=448), dict(dn_value_heads=1, dn_key_heads=1)):
         with pytest.raises(sb.SepalB200Error, match="widths must be multiples of 128"):
             sb.Trunk(0, config(**bad))
 
