@@ -57,7 +57,8 @@ SEPAL_B200_API const char* sepal_b200_last_error(void);
 /* Creates the per-device state every launcher needs: device properties, the scratch memory of the split-k schedule
  * (`workspace_bytes`, 0 = two 128 x 256 float32 tiles per SM, about 39 MB on a B200) and the device status word. All device
  * memory the launchers ever use is allocated here, as the engine allocates its call buffers once (runner/cuda/src/cuda_engine.cpp:714-743).
- * One context serves one stream at a time: launches that overlap on the device must use different contexts.
+ * One context serves one stream at a time: launches that overlap on the device must use different contexts. A call that takes a context
+ * makes the context's device the calling thread's current one, as this call does; those that take none run on the current device.
  * On failure *out is NULL. Counterpart of the engine creation behind sepal_open, c_api.h:39. */
 SEPAL_B200_API int32_t sepal_b200_open(int32_t device, uint64_t workspace_bytes, sepal_b200_ctx** out);
 

@@ -4,8 +4,8 @@
 // operand is converted on its way (the kernels of gemm_tc.cu widen an int8 weight first), so a k step is a load and four MMAs of K 32.
 // And integer addition has no order: however k is cut, the sums, and with them the result's bits, are the same.
 //
-// Both kernels put the weights on the MMA's M side and the tokens on its N side, whose width is free in steps of 16 (pairs: 32), so
-// nothing is computed for tokens that are not there.
+// Both kernels put the weights on the MMA's M side and the tokens on its N side, whose width is free in steps of 16 (pairs: 32): tokens are
+// padded to whole tiles of that width, the last one too, and not to 128 or 256 rows.
 //
 //   gemm_s8_pair_kernel  CTA pairs, 256 weight rows by `bt` tokens to a tile, persistent, two accumulators in tensor memory (the epilogue of a
 //                        tile runs behind the next tile's products).
@@ -15,9 +15,10 @@
 // What bounds them, and what they measured (launches back to back, weights from DRAM, clocks as they were):
 //   - Full calls are bound by the tensor cores under the power cap: 4096 x 24576 x 4096 with SwiGLU 251 us in bursts (3.28 POP/s, where the
 //     measured binary16 rate of the library product, doubled, is 3.31) and 270 to 280 over a quarter of a second.
-//   - A few hundred tokens make one to five waves of tiles; a step takes the 2 bt clocks of its MMAs (310 to 316 measured at bt 160), and what
-//     is lost is the part of the last wave without tiles and about 10,000 clocks a launch: 3000 until the launch before has ended, 1100 for
-//     the first boxes, 4100 for the last tile's results (all pairs add theirs at once; leaving them lane by lane without the staging
+//   - A few hundred tokens make one to five waves of tiles; a step takes about the 2 bt clocks of its MMAs (317 measured alone at bt 160; within
+//     a launch 310 to 316 from one issue to the next, the last MMAs still queued at the end), and what is lost is the part of the last wave
+//     without tiles and about 10,000 clocks a launch: 3000 until the launch before has ended, 1100 for the first boxes, 4100 for the last
+//     tile's results (all pairs add theirs at once, to a Y that comes from DRAM then; leaving them lane by lane without the staging
 //     boxes takes as long, and longer in binary16) and 1400 to leave. 900 x 2560 x 9728 added: 20.3 us (2.2 POP/s); 1337 x 6144 x 2560
 //     16.9; 900 x 19456 x 2560 SwiGLU 36.
 //   - Few tokens are bound by the launch (3.3 us with next to nothing to do) and then the reading of W: one token by 6144 x 2560 5.6 us, 2560 x 9728
@@ -673,7 +674,9 @@ void launch_pair(const Context& ctx, const std::int8_t* x, std::size_t ld_x, con
     const unsigned fixed = 1024 + kEpilogueWarps * 2 * kBoxBytes + kPairTail, stage_bytes = kWBytes + bt / 2 * kBK;
     p.stages = (kSmemMax - fixed) / stage_bytes;
     if (p.stages > kMaxStages) p.stages = kMaxStages;
-    // A binary16 residual update is read and rounded again: lane by lane. And a TMA store drops what lies past the matrix in units of 16 bytes
+    // A binary16 residual update is one float32 addition to the old value, rounded once, where the TMA's binary16 addition would round the product
+    // first: read and written lane by lane, a column to a lane. That is what such a call costs on pairs: 900 x 2560 x 9728 62 us, 24 added to
+    // float32, 22 stored in binary16. (The few-rows kernel adds along rows: 29 x 2560 x 9728 8.5 us, 8.7 to float32.) And a TMA store drops what lies past the matrix in units of 16 bytes
     // only: rows whose length is not a multiple of that would have their next columns overwritten.
     const std::size_t columns = p.epilogue == 2 ? p.n / 2 : p.n;
     p.staged = p.vec_ok != 0 && columns * (p.y_half != 0 ? 2 : 4) % 16 == 0 && !(p.epilogue == 1 && p.y_half != 0) ? 1u : 0u;
@@ -711,7 +714,9 @@ void launch_few(const Context& ctx, const std::int8_t* x, std::size_t ld_x, cons
 
 // The automatic choice: the kernel, and the pair kernel's tokens to a tile, by an estimate in microseconds fitted to every width and every split
 // of k over thirteen projections (1024 to 24576 weight rows, k from 1024 to 12288) at 21 token counts from 1 to 4096 on 148 SMs: what it
-// picks is on average 2 % slower than the best of them, on single shapes of a few microseconds up to 33 %.
+// picks is on average 2 % slower than the best of them, on single shapes of a few microseconds up to 33 %. On six products outside that set (2560
+// x 9216, 18432 x 2560, 12288 x 2048, 2048 x 6144, 5120 x 5120, 1500 x 2000) at seven counts up to 2048 also 2 %, at worst 18 (300 tokens by 1500
+// x 2000; 10 elsewhere). The clock (1900 MHz) and the memory's rate are in it; a binary16 residual update's slower stores are not.
 //   - A step of the pair kernel is 2 bt clocks of tensor cores, or 180 + 0.6 bt where the boxes' arrival bounds it (tiles under 128 tokens); a
 //     wave of tiles has about 600 clocks of its own (first boxes, the last tile's epilogue).
 //   - Cutting k over a cluster costs 0.028 us a token in the exchange of the sums: it wins where a few weight rows have a long k (2560 x 9728, one

@@ -171,7 +171,8 @@ __device__ __forceinline__ unsigned largest_of(unsigned top, const float4& u) {
 }
 
 // DELTA: 0 none, 1 binary16, 2 float32. A vector is four values. WIDE: blocks of more than kNarrowThreads, held to registers that let two
-// of them onto an SM (12288 float32 values a row, 4096 rows: 63 us with one, 46 with two); narrow blocks are faster with all they ask for.
+// of them onto an SM (12288 float32 values a row, 4096 rows: 63 us with one, 46 with two); narrow blocks are faster with all they ask for. (At 40
+// registers the float32 delta's form without values spills 16 bytes; no other does.)
 template <int DELTA, bool WIDE, bool VALUES>
 __global__ void __launch_bounds__(WIDE ? kMaxThreads : kNarrowThreads, WIDE ? 2 : 1) rms_norm_s8_kernel(const RowsParams p) {
     ptx::grid_launch_dependents();
