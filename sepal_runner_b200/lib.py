@@ -863,6 +863,8 @@ def gemm_f16_noalloc(x, w, y, *, epilogue: int = STORE, stream=None, wait: bool 
     n = w.shape[0]
     if w.shape[1] != k or w.device != x.device:
         raise ValueError(f"x is [{t}, {k}] but w is {tuple(w.shape)} on {w.device}: the inner dimensions and the devices must agree")
+    if not x.is_cuda or x.get_device() != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {x.device}: this call runs on the current device and reads its memory only")
     Context._out(x, n // 2 if epilogue == SWIGLU else n, y, y.dtype == torch.float16)
     status = _i32(0)
     _check(library().sepal_b200_gemm_f16_noalloc(x.data_ptr(), x.stride(0) if t > 1 else max(x.stride(0), k), w.data_ptr(),

@@ -115,7 +115,7 @@ def test_a_stream_of_another_device_is_refused(recorded):
     assert calls == []
 
 
-def test_tensors_of_another_device_are_refused(recorded):
+def test_tensors_of_another_device_are_refused(recorded, monkeypatch):
     """Every launching call with tensors that are not on the context's device: an address that its kernel could not read."""
     ctx, calls = recorded
     calls_here = []
@@ -138,6 +138,11 @@ def test_tensors_of_another_device_are_refused(recorded):
         with pytest.raises(ValueError, match="cuda:0"):
             call()
     assert calls == [] and len(calls_here) == 16
+    # the call without a context, which runs on the current device
+    monkeypatch.setattr(binding, "library", lambda: ctx._lib)
+    with pytest.raises(ValueError, match="this call runs on the current device"):
+        sb.gemm_f16_noalloc(h(4, 128), h(8, 128), f(4, 8), stream=types.SimpleNamespace(cuda_stream=0), wait=False)
+    assert calls == []
     ctx.device = DEVICE
     for bad in (torch.zeros(8, dtype=torch.float16), torch.zeros(4, 4).t()[:2]):
         with pytest.raises(AssertionError):
